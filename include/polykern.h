@@ -429,6 +429,83 @@ PK_API int pk_attn_dscores_gemm(int dtype, int degree, int64_t batch, int64_t M,
                                 void* stream);
 
 /*
+ * Token operators (no counterpart in the reference).
+ *
+ * pk_qk_norm_rope_fwd: per-head RMS norm of queries and keys and the position rotation in one pass,
+ *   v = x (*) rsqrt(mean(x (*) x) + eps) (*) w over the head dimension, y = R(position) v.
+ *   x planes [batch][len][heads][dim] with strides (bs, ts, hs) and unit feature stride; y planes
+ *   [batch][heads][len][dim], contiguous (attention's operand).  w: qw_planes / kw_planes planes of
+ *   dim values (0: no weight; fewer than degree + 1: the missing ones are zero).  R turns feature
+ *   pairs of the first `rotary` (even) features, (j, j + rotary/2) or with interleaved != 0
+ *   (2j, 2j + 1), by the angle with cosine cos_t[position][j] and sine sin_t[position][j]
+ *   (tables [table_rows][rotary/2], float, double for PK_F64).  The position of token t of batch
+ *   entry b is positions[b * pos_bs + t], or t when positions is null; a position outside the table
+ *   gives NaN.  q_heads or k_heads may be 0 (that side is skipped).  dim <= 1024.
+ * pk_qk_norm_rope_bwd: dq, dk [batch][len][heads][dim] (contiguous) from the gradients of the outputs
+ *   (strides bs, hs, ts, unit feature stride), and the first qw_planes / kw_planes planes of the
+ *   weights' gradients where dqw / dkw are not null; these are summed in a fixed order through
+ *   workspace (pk_qk_norm_rope_bwd_workspace_size bytes, 0 planes for a null pointer).
+ */
+PK_API int pk_qk_norm_rope_fwd(int dtype, int degree, int64_t batch, int64_t len, int64_t q_heads,
+                               int64_t k_heads, int64_t dim, int64_t rotary, int interleaved,
+                               const void* const* q, int64_t q_bs, int64_t q_ts, int64_t q_hs,
+                               const void* const* k, int64_t k_bs, int64_t k_ts, int64_t k_hs,
+                               const void* const* qw, int qw_planes, const void* const* kw, int kw_planes,
+                               const void* cos_t, const void* sin_t, int64_t table_rows,
+                               const int64_t* positions, int64_t pos_bs, double eps,
+                               void* const* q_out, void* const* k_out, void* stream);
+PK_API size_t pk_qk_norm_rope_bwd_workspace_size(int dtype, int degree, int64_t batch, int64_t len,
+                                                 int64_t q_heads, int64_t k_heads, int64_t dim,
+                                                 int dqw_planes, int dkw_planes);
+PK_API int pk_qk_norm_rope_bwd(int dtype, int degree, int64_t batch, int64_t len, int64_t q_heads,
+                               int64_t k_heads, int64_t dim, int64_t rotary, int interleaved,
+                               const void* const* q, int64_t q_bs, int64_t q_ts, int64_t q_hs,
+                               const void* const* k, int64_t k_bs, int64_t k_ts, int64_t k_hs,
+                               const void* const* qw, int qw_planes, const void* const* kw, int kw_planes,
+                               const void* cos_t, const void* sin_t, int64_t table_rows,
+                               const int64_t* positions, int64_t pos_bs, double eps,
+                               const void* const* gq, int64_t gq_bs, int64_t gq_hs, int64_t gq_ts,
+                               const void* const* gk, int64_t gk_bs, int64_t gk_hs, int64_t gk_ts,
+                               void* const* dq, void* const* dk, void* const* dqw, void* const* dkw,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * pk_dropout: y_k = residual_k + keep * scale * x_k for every plane, one mask for all planes and
+ * never stored.  Element i (row-major over n contiguous elements) is kept when word i % 4 of
+ * Philox4x32-10 with counter (i / 4, offset) and key seed is >= threshold (0 .. 2^32; drop
+ * probability threshold / 2^32).  Planes of x and of the residual past x_planes / residual_planes
+ * are zero.  A dropped element is 0 whatever x holds.  y may be x or residual.
+ */
+PK_API int pk_dropout(int dtype, int degree, int64_t n, const void* const* x, int x_planes,
+                      const void* const* residual, int residual_planes, uint64_t threshold, double scale,
+                      uint64_t seed, uint64_t offset, void* const* y, void* stream);
+
+/*
+ * pk_token_log_probs_fwd: for each row of logits (cols values, row stride logits_rs) of
+ * z = scale * logits, the log probability series of tokens[row], the entropy series
+ * -sum p (*) log p, and the `top` (<= 32) largest logits (ties to the lowest index, NaN above all)
+ * with their log probability series.  Outputs are float (double for PK_F64): log_probs, entropy
+ * [rows]; top_log_probs, top_tokens [rows][top]; stats [rows][degree + 2] for the backward.
+ *   A logit of -inf is masked: no part in any sum, log probability -inf, no direction.  A row with no
+ *   open logit: entropy 0.  A row whose token is ignore_index is not read: zeros, top_tokens -1.  A
+ *   token outside [0, cols) gives NaN.
+ * pk_token_log_probs_bwd: dlogits from the gradients of log_probs, entropy and top_log_probs (null
+ *   arrays: zero), with the forward's stats, entropy and top_tokens.
+ */
+PK_API int pk_token_log_probs_fwd(int dtype, int degree, int64_t rows, int64_t cols,
+                                  const void* const* logits, int64_t logits_rs, const int64_t* tokens,
+                                  int64_t ignore_index, double scale, int top, void* const* log_probs,
+                                  void* const* entropy, void* const* top_log_probs, int64_t* top_tokens,
+                                  void* stats, void* stream);
+PK_API int pk_token_log_probs_bwd(int dtype, int degree, int64_t rows, int64_t cols,
+                                  const void* const* logits, int64_t logits_rs, const int64_t* tokens,
+                                  int64_t ignore_index, double scale, int top, const void* stats,
+                                  const void* const* entropy, const int64_t* top_tokens,
+                                  const void* const* g_log_probs, const void* const* g_entropy,
+                                  const void* const* g_top_log_probs, void* const* dlogits,
+                                  int64_t dlogits_rs, void* stream);
+
+/*
  * pk_poly_gemm without a workspace argument, for callers that cannot allocate device
  * memory (a plugin host that owns every allocation, a process that must not grow its
  * device footprint after start-up, code with no allocator to link).  The scratch comes

@@ -94,6 +94,18 @@ SIGNATURES = {
     "pk_attn_dscores_gemm": (_i32, [_i32, _i32, _i64, _i64, _i64, _i64, _pp, _i64, _i64, _i64,
                                     _pp, _i64, _i64, _i64, _pp, _i64, _i64,
                                     _vp, _i64, ctypes.c_double, _i32, _i64, _pp, _i64, _i64, _vp]),
+    "pk_qk_norm_rope_fwd": (_i32, [_i32, _i32] + [_i64] * 6 + [_i32] + 2 * [_pp, _i64, _i64, _i64]
+                            + 2 * [_pp, _i32] + [_vp, _vp, _i64, _vp, _i64, ctypes.c_double, _pp, _pp, _vp]),
+    "pk_qk_norm_rope_bwd_workspace_size": (_sz, [_i32, _i32] + [_i64] * 5 + [_i32, _i32]),
+    "pk_qk_norm_rope_bwd": (_i32, [_i32, _i32] + [_i64] * 6 + [_i32] + 2 * [_pp, _i64, _i64, _i64]
+                            + 2 * [_pp, _i32] + [_vp, _vp, _i64, _vp, _i64, ctypes.c_double]
+                            + 2 * [_pp, _i64, _i64, _i64] + [_pp, _pp, _pp, _pp, _vp, _sz, _vp]),
+    "pk_dropout": (_i32, [_i32, _i32, _i64, _pp, _i32, _pp, _i32, ctypes.c_uint64, ctypes.c_double,
+                          ctypes.c_uint64, ctypes.c_uint64, _pp, _vp]),
+    "pk_token_log_probs_fwd": (_i32, [_i32, _i32, _i64, _i64, _pp, _i64, _vp, _i64, ctypes.c_double, _i32,
+                                      _pp, _pp, _pp, _vp, _vp, _vp]),
+    "pk_token_log_probs_bwd": (_i32, [_i32, _i32, _i64, _i64, _pp, _i64, _vp, _i64, ctypes.c_double, _i32,
+                                      _vp, _pp, _vp, _pp, _pp, _pp, _pp, _i64, _vp]),
     "pk_poly_gemm_noalloc": (_i32, [_i32, _i32, _i64, _i64, _i64, _i64,
                                     _pp, _i64, _i64, _i64,
                                     _pp, _i64, _i64, _i64,

@@ -266,6 +266,37 @@ class PolyTensor(torch.Tensor):
         return linear_cross_entropy(input, weight, target, ignore_index=ignore_index, reduction=reduction,
                                     softcap=softcap, chunk_rows=chunk_rows)
 
+    @staticmethod
+    def qk_norm_rope(query, key, query_weight, key_weight, cos, sin, positions=None, eps=1e-6, interleaved=False,
+                     check_indices=True):
+        """Queries (B, T, H, D) and keys (B, T, K, D) normalised per head and rotated by position in
+        one pass, returned head-major for attention (see ``_token_ops.qk_norm_rope``).  Accepts
+        ordinary tensors and PolyTensors (no counterpart in the reference)."""
+        from ._token_ops import qk_norm_rope
+
+        return qk_norm_rope(query, key, query_weight, key_weight, cos, sin, positions=positions, eps=eps,
+                            interleaved=interleaved, check_indices=check_indices)
+
+    @staticmethod
+    def dropout(input, p, seed, offset=0, residual=None):
+        """``residual + dropout(input)`` with a mask that is a function of (seed, offset) and the
+        element's index, the same for every coefficient, formed again in backward (see
+        ``_token_ops.dropout``).  Accepts ordinary tensors and PolyTensors (no counterpart in the
+        reference)."""
+        from ._token_ops import dropout
+
+        return dropout(input, p, seed, offset=offset, residual=residual)
+
+    @staticmethod
+    def token_log_probs(logits, tokens, top=0, temperature=1.0, ignore_index=-100, check_indices=True):
+        """Log probabilities of given tokens, entropy and best alternatives of (..., V) logits in one
+        pass, differentiable (see ``_token_ops.token_log_probs``).  Accepts ordinary tensors and
+        PolyTensors (no counterpart in the reference)."""
+        from ._token_ops import token_log_probs
+
+        return token_log_probs(logits, tokens, top=top, temperature=temperature, ignore_index=ignore_index,
+                               check_indices=check_indices)
+
     def backward(self, gradient=None, retain_graph=None, create_graph=False, inputs=None):
         """Reverse-mode through the series: the seed is ``gradient`` as a PolyTensor of this degree
         (an ordinary tensor is its constant term); with no gradient, a real scalar seeds 1."""
