@@ -14,7 +14,7 @@
 // rounded once, when they are stored.
 #include <algorithm>
 
-#include "pk_rows.cuh"
+#include "pk_vec.cuh"
 
 namespace pk {
 
@@ -283,94 +283,645 @@ __global__ void __launch_bounds__(256) qk_norm_rope_bwd_kernel(const RopeParams 
     }
 }
 
-struct WeightSumParams {
-    const void* partial;   // [blocks][nw][D]
-    void* dw[PK_MAX_PLANES];
-    int64_t blocks;
-    int nw, dim;
+// ---------------------------------------------------------------------------------------------
+// Vector form: a row lives in the registers of `lanes` threads (a power of two up to 32; several rows
+// share a warp), each holding one slot: V feature pairs, all planes, read once.  With half-split pairs
+// a slot is two V-element vectors rotary/2 apart, with adjacent pairs 2V consecutive elements, so both
+// members of a pair are in one thread and the rotation needs no exchange; features past `rotary` form
+// slots of 2V consecutive elements with angle 0.  The planes stay in their storage type until they are
+// worked on (16-bit planes take half the registers), and two neighbouring pairs go through packed float
+// arithmetic together: the neighbours of a loaded vector already share a register pair, and so do their
+// angles.  The feature weights wait in shared memory in slot order.
+struct RowShape {
+    int v = 0, lanes = 0, slots = 0;    // v == 0: the scalar form
+    Divisor by_heads[2], by_len;
 };
 
+template <int V>
+struct SlotAt {
+    int a, b;           // first features of the slot's two vectors
+    int angle;          // first pair, or -1: not turned
+    __device__ __forceinline__ SlotAt(const RopeParams& p, int slot) {
+        const int turned = p.rotary / (2 * V);
+        if (slot >= turned) {
+            a = p.rotary + 2 * V * (slot - turned);
+            b = a + V;
+            angle = -1;
+        } else {
+            a = p.interleaved ? 2 * V * slot : V * slot;
+            b = p.interleaved ? a + V : a + p.rotary / 2;
+            angle = V * slot;
+        }
+    }
+    // feature of the first (m == 0) or second member of pair j
+    __device__ __forceinline__ int feature(bool interleaved, int j, int m) const {
+        if (interleaved) return a + 2 * j + m;
+        return (m ? b : a) + j;
+    }
+};
+
+// Degrees up to 5 have kernels of their own, the higher ones share one with planes to spare.
+template <int NP>
+__device__ __forceinline__ bool plane_live(int k, int np) {
+    return NP <= 6 || k < np;
+}
+
+// The V pairs of a slot, all planes: first members in lo, second members in hi.
+template <int NP, typename T, int V>
+struct Slot {
+    using C = typename Compute<T>::type;
+    Raw<T, V> lo[NP], hi[NP];
+
+    // All loads are issued before anything reads them: a test between two planes' loads makes the second
+    // wait for the first (measured so: 837 instead of 403 us at 4 x 2048 tokens, 2 x 16 heads of 128,
+    // degree 3, float32 backward).
+    __device__ __forceinline__ void load(const void* const* planes, int np, int64_t off, const SlotAt<V>& at) {
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+            if constexpr (NP > 6) lo[k] = hi[k] = Raw<T, V>{};
+            if (plane_live<NP>(k, np)) {
+                const T* src = static_cast<const T*>(planes[k]) + off;
+                lo[k] = *reinterpret_cast<const Raw<T, V>*>(src + at.a);
+                hi[k] = *reinterpret_cast<const Raw<T, V>*>(src + at.b);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(void* const* planes, int np, int64_t off, const SlotAt<V>& at) const {
+#pragma unroll
+        for (int k = 0; k < NP; ++k)
+            if (plane_live<NP>(k, np)) {
+                T* dst = static_cast<T*>(planes[k]) + off;
+                *reinterpret_cast<Raw<T, V>*>(dst + at.a) = lo[k];
+                *reinterpret_cast<Raw<T, V>*>(dst + at.b) = hi[k];
+            }
+    }
+    // 2V consecutive elements into pairs of neighbours, and back
+    __device__ __forceinline__ void part() {
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+            const Raw<T, V> c = lo[k], d = hi[k];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                lo[k].set_bits(j, 2 * j < V ? c.bits((2 * j) % V) : d.bits((2 * j) % V));
+                hi[k].set_bits(j, 2 * j + 1 < V ? c.bits((2 * j + 1) % V) : d.bits((2 * j + 1) % V));
+            }
+        }
+    }
+    __device__ __forceinline__ void join() {
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+            const Raw<T, V> c = lo[k], d = hi[k];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                lo[k].set_bits(j, j % 2 ? d.bits(j / 2) : c.bits(j / 2));
+                hi[k].set_bits(j, (V + j) % 2 ? d.bits((V + j) / 2) : c.bits((V + j) / 2));
+            }
+        }
+    }
+    // neighbours 2i and 2i + 1 of the first / second members as a series
+    __device__ __forceinline__ void firsts(int i, Two<C> (&x)[NP]) const {
+#pragma unroll
+        for (int k = 0; k < NP; ++k) x[k] = lo[k].get(i);
+    }
+    __device__ __forceinline__ void seconds(int i, Two<C> (&x)[NP]) const {
+#pragma unroll
+        for (int k = 0; k < NP; ++k) x[k] = hi[k].get(i);
+    }
+    __device__ __forceinline__ void set(int i, const Two<C> (&a)[NP], const Two<C> (&b)[NP]) {
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+            lo[k].set(i, a[k]);
+            hi[k].set(i, b[k]);
+        }
+    }
+};
+
+// The angles of a slot's pairs, two neighbours at a time.
+template <int V, typename C>
+struct Angles {
+    Two<C> c[V / 2], s[V / 2];
+    __device__ __forceinline__ void load(const RopeParams& p, int64_t pos, int angle) {
+        if (pos < 0 || pos >= p.table_rows) {
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) c[i] = s[i] = Two<C>(C(NAN));
+        } else if (angle < 0) {
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                c[i] = Two<C>(C(1));
+                s[i] = Two<C>(C(0));
+            }
+        } else {
+            const int64_t at = pos * (p.rotary / 2) + angle;
+            C u[V], v[V];
+            load_vec<C, V, C>(static_cast<const C*>(p.cos_t) + at, u);
+            load_vec<C, V, C>(static_cast<const C*>(p.sin_t) + at, v);
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                c[i] = Two<C>(u[2 * i], u[2 * i + 1]);
+                s[i] = Two<C>(v[2 * i], v[2 * i + 1]);
+            }
+        }
+    }
+    // (a, b) turned by the angles of pair neighbours i, on every plane; `back` the other way
+    template <int NP>
+    __device__ __forceinline__ void turn(int i, bool back, Two<C> (&a)[NP], Two<C> (&b)[NP]) const {
+        const Two<C> minus = s[i] * Two<C>(C(-1));
+        const Two<C> up = back ? minus : s[i], down = back ? s[i] : minus;
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+            const Two<C> u = fma2(b[k], down, a[k] * c[i]);
+            b[k] = fma2(a[k], up, b[k] * c[i]);
+            a[k] = u;
+        }
+    }
+};
+
+// Weights of a slot's pair neighbours: first members, second members.
+template <typename C>
+struct alignas(2 * sizeof(Two<C>)) Weight {
+    Two<C> lo, hi;
+};
+
+// Feature weights in slot order, [plane][neighbours i][slot]; planes past nw are zero.
+template <int NP, typename T, int V, typename C>
+__device__ __forceinline__ void stage_weights(const RopeParams& p, const HeadSet& set, int slots, Weight<C>* to) {
+    if (set.nw == 0) return;
+    for (int i = threadIdx.x; i < NP * (V / 2) * slots; i += blockDim.x) {
+        const int slot = i % slots, j = i / slots % (V / 2), k = i / (slots * (V / 2));
+        const SlotAt<V> at(p, slot);
+        const T* w = static_cast<const T*>(set.w[k < set.nw ? k : 0]);
+        const auto value = [&](int pair, int m) {
+            return k < set.nw ? to_c<C>(w[at.feature(p.interleaved, pair, m)]) : C(0);
+        };
+        to[i].lo = Two<C>(value(2 * j, 0), value(2 * j + 1, 0));
+        to[i].hi = Two<C>(value(2 * j, 1), value(2 * j + 1, 1));
+    }
+}
+
+// (a, b) (*) w for pair neighbours i of a slot; a weight without directions scales every plane.
+template <int NP, int V, typename C>
+__device__ __forceinline__ void weigh(const Weight<C>* w, int nw, int slots, int slot, int i, Two<C> (&a)[NP], Two<C> (&b)[NP]) {
+    if (nw == 1) {
+        const Weight<C> f = w[i * slots + slot];
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+            a[k] = a[k] * f.lo;
+            b[k] = b[k] * f.hi;
+        }
+    } else if (nw > 1) {
+        Two<C> f[NP], g[NP];
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+            const Weight<C> t = w[(k * (V / 2) + i) * slots + slot];
+            f[k] = t.lo;
+            g[k] = t.hi;
+        }
+        pair_mul<NP, C>(a, f, a);
+        pair_mul<NP, C>(b, g, b);
+    }
+}
+
+template <int NP, typename C>
+__device__ __forceinline__ void group_sum(int lanes, C (&v)[NP]) {
+    for (int off = lanes >> 1; off > 0; off >>= 1) {
+#pragma unroll
+        for (int k = 0; k < NP; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], off);
+    }
+}
+
+// cross += sum over i < k - i of x_i x_(k-i), diag += x_(k/2)^2: x (*) x = 2 cross + diag
+template <int NP, typename C>
+__device__ __forceinline__ void pair_square_acc(const Two<C> (&x)[NP], Two<C> (&cross)[NP], Two<C> (&diag)[NP]) {
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+#pragma unroll
+        for (int i = 0; 2 * i < k; ++i) cross[k] = fma2(x[i], x[k - i], cross[k]);
+        if (k % 2 == 0) diag[k] = fma2(x[k / 2], x[k / 2], diag[k]);
+    }
+}
+
+// The mean of x (*) x over the row, and its r.
+template <int NP, typename C>
+__device__ __forceinline__ void row_rsqrt(const RopeParams& p, int lanes, const Two<C> (&cross)[NP], const Two<C> (&diag)[NP], C (&r)[NP]) {
+    C s[NP];
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+        C a, b;
+        fma2(cross[k], Two<C>(C(2)), diag[k]).get(a, b);
+        s[k] = a + b;
+    }
+    group_sum<NP, C>(lanes, s);
+    const C inv = C(1) / C(p.dim);
+#pragma unroll
+    for (int k = 0; k < NP; ++k) s[k] *= inv;
+    s[0] += C(p.eps);
+    s_rsqrt<NP, C>(s, r);
+}
+
+constexpr int ROPE_THREADS = 128;
+
+// Where a block's rows are: the blocks below q_blocks take the queries' rows, the others the keys', in
+// strides of all their blocks, so that plane pointers and weights are the same for a whole block.
+struct BlockRows {
+    int which;
+    uint32_t first, stride, rows, heads;
+    __device__ __forceinline__ BlockRows(const RopeParams& p, int q_blocks, int lanes) {
+        which = static_cast<int>(blockIdx.x) >= q_blocks ? 1 : 0;
+        heads = static_cast<uint32_t>(p.set[which].heads);
+        rows = static_cast<uint32_t>(p.batch * p.len) * heads;
+        first = (blockIdx.x - (which ? q_blocks : 0)) * (ROPE_THREADS / lanes);
+        stride = (which ? gridDim.x - q_blocks : q_blocks) * (ROPE_THREADS / lanes);
+    }
+};
+
+// Persistent: the weights are staged once per block.
+template <typename T, int NP, int V>
+__global__ void __launch_bounds__(ROPE_THREADS) qk_norm_rope_fwd_vec_kernel(const __grid_constant__ RopeParams p, const RowShape shape, int q_blocks) {
+    using C = typename Compute<T>::type;
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int lanes = shape.lanes, slots = shape.slots;
+    const BlockRows mine(p, q_blocks, lanes);
+    const HeadSet& set = p.set[mine.which];
+    Weight<C>* weights = reinterpret_cast<Weight<C>*>(smem);
+    stage_weights<NP, T, V, C>(p, set, slots, weights);
+    __syncthreads();
+    const uint32_t len = static_cast<uint32_t>(p.len);
+    const int sub = threadIdx.x & (lanes - 1);
+    const SlotAt<V> at(p, sub);
+    const bool inter = p.interleaved != 0;
+    // every thread of a warp takes the same number of steps (the sums below need the whole warp)
+    for (uint32_t first = mine.first; first < mine.rows; first += mine.stride) {
+        const uint32_t row = first + threadIdx.x / lanes;
+        const bool live = sub < slots && row < mine.rows;
+        const uint32_t token = shape.by_heads[mine.which].divide(row), h = row - token * mine.heads;
+        const uint32_t b = shape.by_len.divide(token), t = token - b * len;
+        Slot<NP, T, V> x;
+        Angles<V, C> angles;
+        Two<C> cross[NP], diag[NP];
+#pragma unroll
+        for (int k = 0; k < NP; ++k) cross[k] = diag[k] = Two<C>(C(0));
+        if (live) {
+            x.load(set.x, p.np, b * set.bs + t * set.ts + h * set.hs, at);
+            angles.load(p, position_of(p, b, t), at.angle);
+            if (inter) x.part();
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                Two<C> e[NP];
+                x.firsts(i, e);
+                pair_square_acc<NP, C>(e, cross, diag);
+                x.seconds(i, e);
+                pair_square_acc<NP, C>(e, cross, diag);
+            }
+        }
+        C r[NP];
+        row_rsqrt<NP, C>(p, lanes, cross, diag, r);
+        if (!live) continue;
+        Two<C> rr[NP];
+#pragma unroll
+        for (int k = 0; k < NP; ++k) rr[k] = Two<C>(r[k]);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            Two<C> e[NP], f[NP];
+            x.firsts(i, e);
+            x.seconds(i, f);
+            pair_mul<NP, C>(e, rr, e);
+            pair_mul<NP, C>(f, rr, f);
+            weigh<NP, V, C>(weights, set.nw, slots, sub, i, e, f);
+            angles.turn(i, false, e, f);
+            x.set(i, e, f);
+        }
+        if (inter) x.join();
+        x.store(set.out, p.np, ((b * set.heads + h) * p.len + t) * p.dim, at);
+    }
+}
+
+// A thread keeps its slot from row to row, so the weight gradient is summed in registers; groups of a
+// warp are joined by shuffles, warps in turn through shared memory, blocks by the weight-sum kernel,
+// always in the same order.
+//
+// Measured on B200 (4 x 2048 tokens, 2 x 16 heads of 128; bytes are the planes read and written once):
+// forward float32 degree 3 175 us = 6.1 TB/s, bfloat16 degree 3 110 us = 4.9 TB/s; backward 314 us =
+// 5.1 TB/s and 258 us = 3.1 TB/s.  float32 runs near the rate of a copy; the 16-bit backward is
+// bound by its instructions (about 70 packed multiply-adds per pair and the conversions).  Degree 3 needs
+// three blocks per SM to cover its loads (353 us with the two that its 182 registers would allow);
+// asking for more blocks at other degrees spills and loses.
+template <typename T, int NP, int V>
+__global__ void __launch_bounds__(ROPE_THREADS, NP == 4 ? 3 : 1) qk_norm_rope_bwd_vec_kernel(const __grid_constant__ RopeParams p, const RowShape shape, int q_blocks) {
+    using C = typename Compute<T>::type;
+    constexpr bool EXACT = std::is_same<T, C>::value;     // storage holds the turned gradient unrounded
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int lanes = shape.lanes, slots = shape.slots;
+    const BlockRows mine(p, q_blocks, lanes);
+    const HeadSet& set = p.set[mine.which];
+    Weight<C>* weights = reinterpret_cast<Weight<C>*>(smem);
+    stage_weights<NP, T, V, C>(p, set, slots, weights);
+    __syncthreads();
+    const uint32_t len = static_cast<uint32_t>(p.len);
+    const int sub = threadIdx.x & (lanes - 1);
+    const SlotAt<V> at(p, sub);
+    const bool inter = p.interleaved != 0;
+    const int nsum = set.partial ? set.nw : 0;
+    Two<C> acc[NP][V / 2][2];
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) acc[k][i][0] = acc[k][i][1] = Two<C>(C(0));
+    }
+    for (uint32_t first = mine.first; first < mine.rows; first += mine.stride) {
+        const uint32_t row = first + threadIdx.x / lanes;
+        const bool live = sub < slots && row < mine.rows;
+        const uint32_t token = shape.by_heads[mine.which].divide(row), h = row - token * mine.heads;
+        const uint32_t b = shape.by_len.divide(token), t = token - b * len;
+        Slot<NP, T, V> x, g;
+        Angles<V, C> angles;
+        Two<C> cross[NP], diag[NP], mean[NP];
+#pragma unroll
+        for (int k = 0; k < NP; ++k) cross[k] = diag[k] = mean[k] = Two<C>(C(0));
+        if (live) {
+            x.load(set.x, p.np, b * set.bs + t * set.ts + h * set.hs, at);
+            g.load(set.g, p.np, b * set.g_bs + h * set.g_hs + t * set.g_ts, at);
+            angles.load(p, position_of(p, b, t), at.angle);
+            if (inter) {
+                x.part();
+                g.part();
+            }
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                Two<C> e[NP], f[NP], u[NP];
+                g.firsts(i, e);
+                g.seconds(i, f);
+                angles.turn(i, true, e, f);
+                if constexpr (EXACT) g.set(i, e, f);
+                weigh<NP, V, C>(weights, set.nw, slots, sub, i, e, f);
+                x.firsts(i, u);
+                pair_square_acc<NP, C>(u, cross, diag);
+                pair_mul_acc<NP, C>(u, e, mean);
+                x.seconds(i, u);
+                pair_square_acc<NP, C>(u, cross, diag);
+                pair_mul_acc<NP, C>(u, f, mean);
+            }
+        }
+        C m[NP], r[NP], q[NP];
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+            C u, v;
+            mean[k].get(u, v);
+            m[k] = u + v;
+        }
+        group_sum<NP, C>(lanes, m);
+        row_rsqrt<NP, C>(p, lanes, cross, diag, r);
+        if (!live) continue;
+        s_mul<NP, C>(r, r, q);
+        s_mul<NP, C>(q, r, q);
+        s_mul<NP, C>(q, m, q);
+        Two<C> rr[NP], qq[NP];
+        const C minus = C(-1) / C(p.dim);
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+            rr[k] = Two<C>(r[k]);
+            qq[k] = Two<C>(q[k] * minus);       // -(r (*) r (*) r (*) mean)
+        }
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            Two<C> e[2][NP], f[2][NP];
+            x.firsts(i, e[0]);
+            x.seconds(i, e[1]);
+            g.firsts(i, f[0]);
+            g.seconds(i, f[1]);
+            if constexpr (!EXACT) angles.turn(i, true, f[0], f[1]);
+#pragma unroll
+            for (int m2 = 0; m2 < 2; ++m2) {
+                pair_mul<NP, C>(f[m2], rr, f[m2]);          // g' (*) r
+                if (nsum > 1) {                             // (g' (*) r) (*) x
+#pragma unroll
+                    for (int k = 0; k < NP; ++k) {
+#pragma unroll
+                        for (int j = 0; j <= k; ++j) acc[k][i][m2] = fma2(f[m2][j], e[m2][k - j], acc[k][i][m2]);
+                    }
+                } else if (nsum == 1) {
+                    acc[0][i][m2] = fma2(f[m2][0], e[m2][0], acc[0][i][m2]);
+                }
+            }
+            weigh<NP, V, C>(weights, set.nw, slots, sub, i, f[0], f[1]);
+            pair_mul_acc<NP, C>(e[0], qq, f[0]);
+            pair_mul_acc<NP, C>(e[1], qq, f[1]);
+            x.set(i, f[0], f[1]);
+        }
+        if (inter) x.join();
+        x.store(set.out, p.np, static_cast<int64_t>(row) * p.dim, at);
+    }
+    if (nsum == 0) return;
+    __syncthreads();                            // the weights are done with: their place takes the sums
+    C* sums = reinterpret_cast<C*>(smem);
+    const int lane = threadIdx.x & 31, dim = static_cast<int>(p.dim);
+    for (int of = 0; of < ROPE_THREADS / 32; ++of) {
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+            if (k >= nsum) continue;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {       // first members, then second members
+                C u, v;
+                acc[k][i / 2][i % 2].get(u, v);
+                for (int off = lanes; off < 32; off <<= 1) {
+                    u += __shfl_xor_sync(0xffffffffu, u, off);
+                    v += __shfl_xor_sync(0xffffffffu, v, off);
+                }
+                if (static_cast<int>(threadIdx.x >> 5) == of && lane < slots) {
+                    C* to = sums + k * dim;
+                    const int a = at.feature(inter, i / 2 * 2, i % 2), b = at.feature(inter, i / 2 * 2 + 1, i % 2);
+                    to[a] = of ? to[a] + u : u;
+                    to[b] = of ? to[b] + v : v;
+                }
+            }
+        }
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < nsum * dim; i += ROPE_THREADS)
+        static_cast<C*>(set.partial)[static_cast<int64_t>(blockIdx.x - (mine.which ? q_blocks : 0)) * nsum * dim + i] = sums[i];
+}
+
+struct WeightSum {
+    const void* partial;   // [blocks][nw][D]
+    void* dw[PK_MAX_PLANES];
+    int blocks, nw;
+};
+struct WeightSumParams {
+    WeightSum set[2];
+    int dim;
+};
+
+// dw = the sum of the blocks' partial sums: 32 values per block, eight threads for each, which take every
+// eighth partial and are joined in order.
 template <typename T>
 __global__ void __launch_bounds__(256) qk_weight_sum_kernel(const WeightSumParams p) {
     using C = typename Compute<T>::type;
-    const int i = blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= p.nw * p.dim) return;
+    __shared__ C part[8][32];
+    const WeightSum& set = p.set[blockIdx.y];
+    const int count = set.nw * p.dim;
+    const int i = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
     C acc = C(0);
-    for (int64_t b = 0; b < p.blocks; ++b) acc += static_cast<const C*>(p.partial)[b * p.nw * p.dim + i];
-    static_cast<T*>(p.dw[i / p.dim])[i % p.dim] = from_c<T>(acc);
+    if (i < count) {
+#pragma unroll 8
+        for (int b = g; b < set.blocks; b += 8) acc += static_cast<const C*>(set.partial)[static_cast<int64_t>(b) * count + i];
+    }
+    part[g][threadIdx.x & 31] = acc;
+    __syncthreads();
+    if (g == 0 && i < count) {
+        for (int j = 1; j < 8; ++j) acc += part[j][threadIdx.x];
+        static_cast<T*>(set.dw[i / p.dim])[i % p.dim] = from_c<T>(acc);
+    }
 }
 
 constexpr int ROPE_MAX_DIM = 1024;
 
-static int compute_bytes(int dtype) { return dtype == PK_F64 ? 8 : 4; }
+// Whether the register form with NP planes and V-element vectors is built: the planes of a slot take `held`
+// registers, and the backward holds the input's, the gradient's and the weight sums.  Past these
+// limits the compiler spills (degree 3: 16-byte vectors forward and backward for float32, float64; 8-byte
+// ones backward for the 16-bit types).
+constexpr bool vec_built(int np, int v, int compute_bytes, bool backward) {
+    const int held = np * 2 * v * compute_bytes / 4;
+    return v >= 2 && held <= (backward ? 48 : 80);
+}
 
-// Backward launch shape: warps per block so that their weight-gradient planes fit in shared memory,
-// and the blocks of the queries and of the keys in proportion to their rows.
-struct BwdShape {
-    int warps, q_blocks, k_blocks;
-    size_t smem;
-};
-static BwdShape bwd_shape(int dtype, int64_t q_rows, int64_t k_rows, int64_t dim, int planes) {
-    BwdShape s{};
-    const size_t per_warp = static_cast<size_t>(planes) * dim * compute_bytes(dtype);
-    s.warps = 8;
-    while (s.warps > 1 && s.warps * per_warp > 96 * 1024) s.warps /= 2;
-    s.smem = s.warps * per_warp;
-    const int64_t room = static_cast<int64_t>(num_sms()) * 4;
-    const auto blocks = [&](int64_t rows) {
-        if (rows == 0) return static_cast<int64_t>(0);
-        const int64_t share = std::max<int64_t>(1, room * rows / (q_rows + k_rows));
-        return std::min<int64_t>(share, ceil_div(rows, s.warps));
-    };
-    s.q_blocks = static_cast<int>(blocks(q_rows));
-    s.k_blocks = static_cast<int>(blocks(k_rows));
+// Vectors of 16 bytes, else of 8, where that form is built, no pair or passing feature is cut, every base
+// and stride is a multiple of the vector, and a row fits a warp; otherwise the scalar form.
+template <typename T, int NP>
+static RowShape row_shape(const RopeParams& p, bool backward) {
+    RowShape s;
+    constexpr int cb = sizeof(typename Compute<T>::type);
+    const int64_t rows = p.batch * p.len * (p.set[0].heads + p.set[1].heads);
+    for (int bytes = 16; bytes >= 8; bytes /= 2) {
+        const int v = bytes / static_cast<int>(sizeof(T));
+        if (!vec_built(NP, v, cb, backward) || p.rotary % (2 * v) || (p.dim - p.rotary) % (2 * v) || p.dim / (2 * v) > 32)
+            continue;
+        const int table = std::min(16, v * cb);
+        bool ok = rows * 32 < (1ll << 32) && planes_aligned(&p.cos_t, 1, table) && planes_aligned(&p.sin_t, 1, table);
+        for (const HeadSet& set : p.set) {
+            if (set.heads == 0) continue;
+            ok = ok && planes_aligned(set.x, p.np, bytes) && planes_aligned(set.out, p.np, bytes) &&
+                 planes_aligned(set.w, set.nw, bytes) && set.bs % v == 0 && set.ts % v == 0 && set.hs % v == 0;
+            if (backward)
+                ok = ok && planes_aligned(set.g, p.np, bytes) && set.g_bs % v == 0 && set.g_hs % v == 0 && set.g_ts % v == 0;
+        }
+        if (!ok) continue;
+        s.v = v;
+        s.slots = static_cast<int>(p.dim) / (2 * v);
+        s.lanes = 1;
+        while (s.lanes < s.slots) s.lanes *= 2;
+        for (int i = 0; i < 2; ++i) s.by_heads[i] = Divisor(static_cast<uint32_t>(std::max<int64_t>(1, p.set[i].heads)));
+        s.by_len = Divisor(static_cast<uint32_t>(p.len));
+        return s;
+    }
     return s;
 }
 
-template <typename T, int NP>
-static void launch_rope_fwd(const RopeParams& p, cudaStream_t s) {
-    const int64_t rows = p.batch * p.len * (p.set[0].heads + p.set[1].heads);
-    const int grid = static_cast<int>(std::min<int64_t>(ceil_div(rows, 8), static_cast<int64_t>(num_sms()) * 32));
-    PK_LAUNCHED(qk_norm_rope_fwd_kernel<T, NP><<<grid, 256, 0, s>>>(p));
+// The backward runs as many blocks as the GPU holds at a time (more would only add partial weight sums), at
+// most ROPE_SUM_BLOCKS per SM, which is what the workspace has room for.
+constexpr int ROPE_SUM_BLOCKS = 16;
+
+// Blocks of the queries and of the keys, in proportion to their rows: at most `room` (about) together, and
+// no more than have a row.
+struct BlockShare {
+    int q = 0, k = 0;
+    BlockShare() = default;
+    BlockShare(const RopeParams& p, int64_t room, int64_t rows_per_block) {
+        const int64_t q_rows = p.batch * p.len * p.set[0].heads, k_rows = p.batch * p.len * p.set[1].heads;
+        const auto share = [&](int64_t rows) {
+            if (rows == 0) return 0;
+            return static_cast<int>(std::min(std::max<int64_t>(1, room * rows / (q_rows + k_rows)), ceil_div(rows, rows_per_block)));
+        };
+        q = share(q_rows);
+        k = share(k_rows);
+    }
+};
+
+struct BwdLaunch {
+    int sums[2];            // planes of the weight gradients wanted
+    void* workspace;
+    BlockShare blocks;
+
+    template <typename C>
+    void plan(RopeParams& p, int resident, int64_t rows_per_block) {
+        blocks = BlockShare(p, static_cast<int64_t>(std::min(resident, ROPE_SUM_BLOCKS)) * num_sms(), rows_per_block);
+        C* at = static_cast<C*>(workspace);
+        p.set[0].partial = sums[0] ? at : nullptr;
+        p.set[1].partial = sums[1] ? at + static_cast<int64_t>(blocks.q) * sums[0] * p.dim : nullptr;
+    }
+};
+
+template <typename K>
+static int resident_blocks(K kernel, int threads, size_t smem) {
+    int n = 0;
+    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) == cudaSuccess && n > 0 ? n : 1;
+}
+
+template <typename T, int NP, int V>
+static bool launch_rope_vec(RopeParams& p, const RowShape& row, BwdLaunch* bwd, cudaStream_t s) {
+    using C = typename Compute<T>::type;
+    if (row.v != V) return false;
+    const size_t weights = static_cast<size_t>(NP) * (V / 2) * row.slots * sizeof(Weight<C>);
+    const int64_t rows_per_block = ROPE_THREADS / row.lanes;
+    if (bwd) {
+        if constexpr (vec_built(NP, V, sizeof(C), true)) {
+            const auto kernel = qk_norm_rope_bwd_vec_kernel<T, NP, V>;
+            bwd->plan<C>(p, resident_blocks(kernel, ROPE_THREADS, weights), rows_per_block);
+            PK_LAUNCHED(kernel<<<bwd->blocks.q + bwd->blocks.k, ROPE_THREADS, weights, s>>>(p, row, bwd->blocks.q));
+        }
+    } else {
+        if constexpr (vec_built(NP, V, sizeof(C), false)) {
+            const auto kernel = qk_norm_rope_fwd_vec_kernel<T, NP, V>;
+            const BlockShare blocks(p, static_cast<int64_t>(num_sms()) * resident_blocks(kernel, ROPE_THREADS, weights), rows_per_block);
+            PK_LAUNCHED(kernel<<<blocks.q + blocks.k, ROPE_THREADS, weights, s>>>(p, row, blocks.q));
+        }
+    }
+    return true;
 }
 
 template <typename T, int NP>
-static void launch_rope_bwd(const RopeParams& p, const BwdShape& shape, cudaStream_t s) {
-    if (shape.smem > 48 * 1024)
-        cudaFuncSetAttribute(qk_norm_rope_bwd_kernel<T, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(shape.smem));
-    PK_LAUNCHED(qk_norm_rope_bwd_kernel<T, NP>
-                <<<shape.q_blocks + shape.k_blocks, shape.warps * 32, shape.smem, s>>>(p, shape.q_blocks));
+static void launch_rope_np(RopeParams& p, BwdLaunch* bwd, cudaStream_t s) {
+    using C = typename Compute<T>::type;
+    const RowShape row = row_shape<T, NP>(p, bwd != nullptr);
+    if (launch_rope_vec<T, NP, 16 / sizeof(T)>(p, row, bwd, s) || launch_rope_vec<T, NP, 8 / sizeof(T)>(p, row, bwd, s))
+        return;
+    if (bwd) {
+        // as many warps as have room for their weight sums in shared memory
+        const size_t per_warp = static_cast<size_t>(std::max(bwd->sums[0], bwd->sums[1])) * p.dim * sizeof(C);
+        int warps = 8;
+        while (warps > 1 && warps * per_warp > 96 * 1024) warps /= 2;
+        const size_t smem = warps * per_warp;
+        const auto kernel = qk_norm_rope_bwd_kernel<T, NP>;
+        if (smem > 48 * 1024)
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        bwd->plan<C>(p, resident_blocks(kernel, warps * 32, smem), warps);
+        PK_LAUNCHED(kernel<<<bwd->blocks.q + bwd->blocks.k, warps * 32, smem, s>>>(p, bwd->blocks.q));
+    } else {
+        const int64_t rows = p.batch * p.len * (p.set[0].heads + p.set[1].heads);
+        const int grid = static_cast<int>(std::min<int64_t>(ceil_div(rows, 8), static_cast<int64_t>(num_sms()) * 32));
+        PK_LAUNCHED(qk_norm_rope_fwd_kernel<T, NP><<<grid, 256, 0, s>>>(p));
+    }
 }
 
 template <typename T>
-static void launch_rope(const RopeParams& p, const BwdShape* shape, cudaStream_t s) {
-#define PK_ROPE_CASE(NP) \
-    if (shape) launch_rope_bwd<T, NP>(p, *shape, s); \
-    else launch_rope_fwd<T, NP>(p, s); \
-    break
+static void launch_rope(RopeParams& p, BwdLaunch* bwd, cudaStream_t s) {
     switch (p.np) {
-        case 1: PK_ROPE_CASE(1);
-        case 2: PK_ROPE_CASE(2);
-        case 3: PK_ROPE_CASE(3);
-        case 4: PK_ROPE_CASE(4);
-        case 5: PK_ROPE_CASE(5);
-        case 6: PK_ROPE_CASE(6);
-        case 7: case 8: case 9: PK_ROPE_CASE(9);
-        default: PK_ROPE_CASE(16);
+        case 1: launch_rope_np<T, 1>(p, bwd, s); break;
+        case 2: launch_rope_np<T, 2>(p, bwd, s); break;
+        case 3: launch_rope_np<T, 3>(p, bwd, s); break;
+        case 4: launch_rope_np<T, 4>(p, bwd, s); break;
+        case 5: launch_rope_np<T, 5>(p, bwd, s); break;
+        case 6: launch_rope_np<T, 6>(p, bwd, s); break;
+        case 7: case 8: case 9: launch_rope_np<T, 9>(p, bwd, s); break;
+        default: launch_rope_np<T, 16>(p, bwd, s); break;
     }
-#undef PK_ROPE_CASE
 }
 
-static int launch_rope_dtype(int dtype, const RopeParams& p, const BwdShape* shape, cudaStream_t s, const char* what) {
+static void launch_rope_dtype(int dtype, RopeParams& p, BwdLaunch* bwd, cudaStream_t s) {
     switch (dtype) {
-        case PK_F32: launch_rope<float>(p, shape, s); break;
-        case PK_F64: launch_rope<double>(p, shape, s); break;
-        case PK_BF16: launch_rope<__nv_bfloat16>(p, shape, s); break;
-        case PK_F16: launch_rope<__half>(p, shape, s); break;
-        default: return fail(PK_ERR_UNSUPPORTED, std::string(what) + ": unsupported dtype");
+        case PK_F32: launch_rope<float>(p, bwd, s); break;
+        case PK_F64: launch_rope<double>(p, bwd, s); break;
+        case PK_BF16: launch_rope<__nv_bfloat16>(p, bwd, s); break;
+        default: launch_rope<__half>(p, bwd, s); break;
     }
-    return PK_OK;
 }
 
 static int check_planes(const void* const* planes, int n, const char* what) {
@@ -453,9 +1004,8 @@ int pk_qk_norm_rope_fwd(int dtype, int degree, int64_t batch, int64_t len, int64
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     void* tok;
     prof_begin("qk_norm_rope_fwd", s, &tok);
-    const int rc = launch_rope_dtype(dtype, p, nullptr, s, what);
+    launch_rope_dtype(dtype, p, nullptr, s);
     prof_end("qk_norm_rope_fwd", s, tok);
-    if (rc) return rc;
     PK_CHECK_LAUNCH(what);
     return PK_OK;
 }
@@ -466,9 +1016,8 @@ size_t pk_qk_norm_rope_bwd_workspace_size(int dtype, int degree, int64_t batch, 
                    "pk_qk_norm_rope_bwd_workspace_size"))
         return 0;
     if (dqw_planes < 0 || dqw_planes > degree + 1 || dkw_planes < 0 || dkw_planes > degree + 1) return 0;
-    const BwdShape s = bwd_shape(dtype, batch * len * q_heads, batch * len * k_heads, dim,
-                                 std::max(dqw_planes, dkw_planes));
-    return static_cast<size_t>(s.q_blocks * dqw_planes + s.k_blocks * dkw_planes) * dim * compute_bytes(dtype);
+    return static_cast<size_t>(num_sms()) * ROPE_SUM_BLOCKS * std::max(dqw_planes, dkw_planes) * dim *
+           (dtype == PK_F64 ? 8 : 4) + 2 * static_cast<size_t>(dqw_planes + dkw_planes) * dim * 8;
 }
 
 int pk_qk_norm_rope_bwd(int dtype, int degree, int64_t batch, int64_t len, int64_t q_heads, int64_t k_heads,
@@ -508,14 +1057,10 @@ int pk_qk_norm_rope_bwd(int dtype, int degree, int64_t batch, int64_t len, int64
     const int64_t heads[2] = {q_heads, k_heads};
     const int64_t strides[2][6] = {{q_bs, q_ts, q_hs, gq_bs, gq_hs, gq_ts}, {k_bs, k_ts, k_hs, gk_bs, gk_hs, gk_ts}};
     const int sums[2] = {dqw ? qw_planes : 0, dkw ? kw_planes : 0};
-    const BwdShape shape = bwd_shape(dtype, batch * len * q_heads, batch * len * k_heads, dim,
-                                     std::max(sums[0], sums[1]));
-    const int64_t blocks[2] = {shape.q_blocks, shape.k_blocks};
     const size_t need = pk_qk_norm_rope_bwd_workspace_size(dtype, degree, batch, len, q_heads, k_heads, dim, sums[0],
                                                            sums[1]);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(PK_ERR_WORKSPACE, "pk_qk_norm_rope_bwd: workspace missing or too small");
-    size_t used = 0;
     for (int i = 0; i < 2; ++i) {
         HeadSet& s = p.set[i];
         s.heads = heads[i];
@@ -540,34 +1085,31 @@ int pk_qk_norm_rope_bwd(int dtype, int degree, int64_t batch, int64_t len, int64
             s.out[j] = out[i][j];
         }
         for (int j = 0; j < nw[i]; ++j) s.w[j] = w[i][j];
-        if (sums[i]) {
-            s.partial = static_cast<unsigned char*>(workspace) + used;
-            used += static_cast<size_t>(blocks[i]) * sums[i] * dim * compute_bytes(dtype);
-        }
     }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     void* tok;
     prof_begin("qk_norm_rope_bwd", s, &tok);
-    int rc = PK_OK;
-    if (shape.q_blocks + shape.k_blocks > 0) rc = launch_rope_dtype(dtype, p, &shape, s, what);
-    for (int i = 0; i < 2 && rc == PK_OK; ++i) {
-        if (!sums[i]) continue;
-        WeightSumParams q2{};
-        q2.partial = p.set[i].partial;
-        q2.blocks = blocks[i];
-        q2.nw = sums[i];
-        q2.dim = static_cast<int>(dim);
-        for (int j = 0; j < sums[i]; ++j) q2.dw[j] = dw[i][j];
-        const int grid = static_cast<int>(ceil_div(sums[i] * dim, 256));
+    BwdLaunch bwd{{sums[0], sums[1]}, workspace, {}};
+    if (batch * len * (q_heads + k_heads) > 0) launch_rope_dtype(dtype, p, &bwd, s);
+    if (sums[0] + sums[1] > 0) {
+        const int blocks[2] = {bwd.blocks.q, bwd.blocks.k};
+        WeightSumParams total{};
+        total.dim = static_cast<int>(dim);
+        for (int i = 0; i < 2; ++i) {
+            total.set[i].partial = p.set[i].partial;
+            total.set[i].blocks = blocks[i];
+            total.set[i].nw = sums[i];
+            for (int j = 0; j < sums[i]; ++j) total.set[i].dw[j] = dw[i][j];
+        }
+        const dim3 grid(static_cast<unsigned>(ceil_div(std::max(sums[0], sums[1]) * dim, 32)), 2);
         switch (dtype) {
-            case PK_F32: PK_LAUNCHED(qk_weight_sum_kernel<float><<<grid, 256, 0, s>>>(q2)); break;
-            case PK_F64: PK_LAUNCHED(qk_weight_sum_kernel<double><<<grid, 256, 0, s>>>(q2)); break;
-            case PK_BF16: PK_LAUNCHED(qk_weight_sum_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(q2)); break;
-            default: PK_LAUNCHED(qk_weight_sum_kernel<__half><<<grid, 256, 0, s>>>(q2)); break;
+            case PK_F32: PK_LAUNCHED(qk_weight_sum_kernel<float><<<grid, 256, 0, s>>>(total)); break;
+            case PK_F64: PK_LAUNCHED(qk_weight_sum_kernel<double><<<grid, 256, 0, s>>>(total)); break;
+            case PK_BF16: PK_LAUNCHED(qk_weight_sum_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(total)); break;
+            default: PK_LAUNCHED(qk_weight_sum_kernel<__half><<<grid, 256, 0, s>>>(total)); break;
         }
     }
     prof_end("qk_norm_rope_bwd", s, tok);
-    if (rc) return rc;
     PK_CHECK_LAUNCH(what);
     return PK_OK;
 }
