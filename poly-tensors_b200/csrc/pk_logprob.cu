@@ -12,9 +12,12 @@
 //
 // Sums, maxima and the row series are held in float (double for float64 logits); the results have that
 // type, and the gradient is rounded once to the logits' type when it is stored.
-#include <algorithm>
+#include <cooperative_groups.h>
 
-#include "pk_rows.cuh"
+#include <algorithm>
+#include <cstring>
+
+#include "pk_vec.cuh"
 
 namespace pk {
 
@@ -30,6 +33,7 @@ struct LogProbParams {
     void* dx[PK_MAX_PLANES];
     int np, top;
     int has_a, has_b, has_c;
+    int aligned;                         // every plane's base lies alike within 16 bytes
     int64_t rows, cols, x_rs, dx_rs;
     const int64_t* tokens;
     int64_t ignore_index;
@@ -42,69 +46,179 @@ struct LogProbParams {
 
 constexpr int LP_MAX_TOP = 32;
 
-// Running state of a part of a row: the largest z_0 seen, S and T = sum w (*) (z - m) below it.
+__device__ __forceinline__ float exp_fast(float x) {
+    // 2^(x log2 e) in hardware: the argument's rounding, |x| 2^-24, is the same size as the logit's own
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+    return y;
+}
+__device__ __forceinline__ double exp_fast(double x) { return exp(x); }
+// the same with subnormal results (a gradient of 1e-38 is one; a weight of 1e-38 beside a sum of 1 is not)
+__device__ __forceinline__ float exp_small(float x) {
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+    return y;
+}
+__device__ __forceinline__ double exp_small(double x) { return exp(x); }
+
+// Largest value, NaN when there is one.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ double max_nan(double a, double b) { return a != a ? a : b != b ? b : fmax(a, b); }
+
+// Elements of a 16-byte vector.
+template <typename T>
+constexpr int lp_vec() { return 16 / sizeof(T); }
+
+// A row as groups of one vector: group g holds elements g * VEC - skew ..; the first group starts at the
+// 16-byte boundary at or before the row, so that whole groups are aligned whatever the row's offset.
+struct RowGroups {
+    int skew, count;
+    template <typename T>
+    __device__ __forceinline__ void set(const void* row, int64_t cols, bool aligned) {
+        constexpr int VEC = lp_vec<T>();
+        skew = aligned ? static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T)) : 0;
+        count = static_cast<int>((cols + skew + VEC - 1) / VEC);
+    }
+};
+
+// One group of every plane; elements outside the row read as masked (-inf, no direction).
+template <int NP, typename T>
+struct Group {
+    static constexpr int VEC = lp_vec<T>();
+    Raw<T, VEC> v[NP];
+
+    __device__ __forceinline__ void load(const LogProbParams& p, int64_t row_at, const RowGroups& row, int g, bool aligned) {
+        const int64_t first = static_cast<int64_t>(g) * VEC - row.skew;
+        if (aligned && first >= 0 && first + VEC <= p.cols) {
+#pragma unroll
+            for (int k = 0; k < NP; ++k) {
+                if constexpr (NP > 6) v[k] = Raw<T, VEC>{};
+                if (NP <= 6 || k < p.np)
+                    v[k] = *reinterpret_cast<const Raw<T, VEC>*>(static_cast<const T*>(p.x[k]) + row_at + first);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < NP; ++k) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const bool in = first + j >= 0 && first + j < p.cols && (NP <= 6 || k < p.np);
+                    const T e = in ? static_cast<const T*>(p.x[k])[row_at + first + j]
+                                   : from_c<T>(k ? typename Compute<T>::type(0) : typename Compute<T>::type(-INFINITY));
+                    uint64_t bits = 0;
+                    memcpy(&bits, &e, sizeof(T));
+                    v[k].set_bits(j, bits);
+                }
+            }
+        }
+    }
+};
+
+// What a sum leaves behind when its weight underflows: nothing, unless a NaN logit is in it.
+template <typename C>
+__device__ __forceinline__ C nan_or_zero(C v) { return v == v ? C(0) : v; }
+
+// Running state of a part of a row: the largest z_0 seen, S and T = sum w (*) (z - m) below it.  Two sums
+// of each run side by side (even and odd elements) and are joined at the end.
 template <int NP, typename C>
 struct LogSum {
     C m;
-    C S[NP], T[NP];
+    Two<C> S[NP], T[NP];
+    __device__ __forceinline__ void clear() {
+        m = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < NP; ++k) S[k] = T[k] = Two<C>(C(0));
+    }
+    // The same sums below a larger maximum.
+    __device__ __forceinline__ void raise(C to) {
+        const C d = m - to, f = m == -INFINITY ? C(0) : exp_fast(d);
+        if (f == C(0)) {
+#pragma unroll
+            for (int k = 0; k < NP; ++k) {
+                C a, b;
+                S[k].get(a, b);
+                S[k] = Two<C>(nan_or_zero(a), nan_or_zero(b));
+                T[k] = Two<C>(C(0));
+            }
+        } else {
+            const Two<C> ff(f), dd(d);
+#pragma unroll
+            for (int k = 0; k < NP; ++k) {
+                T[k] = ff * fma2(dd, S[k], T[k]);
+                S[k] = ff * S[k];
+            }
+        }
+        m = to;
+    }
+    // Two elements: z holds the constant planes unscaled, u the directions scaled (u[0] unused).
+    __device__ __forceinline__ void add(Two<C> x, C scale, Two<C> (&u)[NP]) {
+        Two<C> d = fma2(x, Two<C>(scale), Two<C>(m == -INFINITY ? C(0) : -m));
+        C d0, d1;
+        d.get(d0, d1);
+        const C w0 = exp_fast(d0), w1 = exp_fast(d1);
+        if (w0 == C(0) || w1 == C(0)) {
+            // masked, or too far below the maximum to count: neither its logit nor its directions enter
+            d = Two<C>(w0 == C(0) ? C(0) : d0, w1 == C(0) ? C(0) : d1);
+#pragma unroll
+            for (int k = 1; k < NP; ++k) {
+                C a, b;
+                u[k].get(a, b);
+                u[k] = Two<C>(w0 == C(0) ? C(0) : a, w1 == C(0) ? C(0) : b);
+            }
+        }
+        const Two<C> w(w0, w1);
+        // e = exp(directions) and q = e (*) directions from the same products u_i e_(k-i)
+        Two<C> e[NP];
+        S[0] = S[0] + w;
+        T[0] = fma2(w, d, T[0]);
+        e[0] = Two<C>(C(1));
+#pragma unroll
+        for (int k = 1; k < NP; ++k) {
+            Two<C> t = u[k], v = u[k];                       // i = k: e_0 = 1
+#pragma unroll
+            for (int i = 1; i < k; ++i) {
+                const Two<C> o = u[i] * e[k - i];
+                t = fma2(o, Two<C>(C(i) / C(k)), t);
+                v = v + o;
+            }
+            e[k] = t;
+            S[k] = fma2(w, t, S[k]);
+            T[k] = fma2(w, fma2(d, t, v), T[k]);
+        }
+    }
+};
+
+// The joined sums of many threads' parts.
+template <int NP, typename C>
+struct RowSum {
+    C m, S[NP], T[NP];
     __device__ __forceinline__ void clear() {
         m = -INFINITY;
 #pragma unroll
         for (int k = 0; k < NP; ++k) S[k] = T[k] = C(0);
     }
-    // The same sums below a larger maximum.
-    __device__ __forceinline__ void raise(C to) {
-        if (m == -INFINITY) {
-            m = to;
-            return;
-        }
-        const C f = c_exp(m - to), d = m - to;
+    // All lanes of the warp: every lane gets the total.  The largest maximum first, then plain sums.
+    __device__ __forceinline__ void join_warp() {
+        C top = m;
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, off));
+        const C d = m - top, f = m == -INFINITY ? C(0) : exp_fast(d);
 #pragma unroll
         for (int k = 0; k < NP; ++k) {
             T[k] = f == C(0) ? C(0) : f * (T[k] + d * S[k]);
-            S[k] = f == C(0) ? C(0) : f * S[k];
+            S[k] = f == C(0) ? nan_or_zero(S[k]) : f * S[k];
         }
-        m = to;
-    }
-    __device__ __forceinline__ void add(const C (&z)[NP]) {
-        if (z[0] == -INFINITY) return;
-        if (!(z[0] <= m)) raise(z[0]);
-        const C d = z[0] - m, w = c_exp(d);
-        if (w == C(0)) return;
-        // e = exp(directions) and q = e (*) directions from the same products u_i e_{k-i}
-        C e[NP], q[NP];
-        e[0] = C(1);
-        q[0] = C(0);
+        m = top;
 #pragma unroll
-        for (int k = 1; k < NP; ++k) {
-            C t = C(0), v = C(0);
+        for (int k = 0; k < NP; ++k) {
 #pragma unroll
-            for (int i = 1; i <= k; ++i) {
-                const C o = z[i] * e[k - i];
-                t += C(i) * o;
-                v += o;
+            for (int off = 16; off > 0; off >>= 1) {
+                S[k] += __shfl_xor_sync(0xffffffffu, S[k], off);
+                T[k] += __shfl_xor_sync(0xffffffffu, T[k], off);
             }
-            e[k] = t * inv_int<C>(k);
-            q[k] = v;
-        }
-#pragma unroll
-        for (int k = 0; k < NP; ++k) {
-            S[k] += w * e[k];
-            T[k] += w * (q[k] + d * e[k]);
-        }
-    }
-    __device__ __forceinline__ void join(const LogSum& o) {
-        if (o.m == -INFINITY) return;
-        if (!(o.m <= m)) {
-            const C om = o.m;
-            raise(om);
-        }
-        LogSum b = o;
-        b.raise(m);
-#pragma unroll
-        for (int k = 0; k < NP; ++k) {
-            S[k] += b.S[k];
-            T[k] += b.T[k];
         }
     }
 };
@@ -137,232 +251,481 @@ __device__ __forceinline__ uint64_t order_key(double v) {
     return b >> 63 ? ~b : b | (1ull << 63);
 }
 
-// One block per row.
-template <typename T, int NP>
-__global__ void __launch_bounds__(256) token_log_probs_fwd_kernel(const LogProbParams p) {
-    using C = typename Compute<T>::type;
-    __shared__ LogSum<NP, C> part[8];
-    __shared__ uint64_t best_key[8];
-    __shared__ int64_t best_at[8];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        const int64_t token = p.tokens[row];
-        if (token == p.ignore_index) {   // not read: zeros, and no alternatives
-            if (threadIdx.x == 0) {
-                for (int k = 0; k < p.np; ++k) {
-                    static_cast<C*>(p.logp[k])[row] = static_cast<C*>(p.entropy[k])[row] = C(0);
-                    for (int j = 0; j < p.top; ++j) static_cast<C*>(p.top_logp[k])[row * p.top + j] = C(0);
-                }
-                for (int j = 0; j < p.top; ++j) p.top_tokens[row * p.top + j] = -1;
-                for (int k = 0; k <= p.np; ++k) static_cast<C*>(p.stats)[row * (p.np + 1) + k] = C(0);
+// A warp's best logits so far: lane j holds the (j + 1)-th in (value falling, index rising) order.
+template <typename C>
+struct Best {
+    uint64_t key;
+    int at;
+    C bar;          // a value below this cannot enter the first `top`
+    __device__ __forceinline__ void clear() {
+        key = 0;
+        at = 0x7fffffff;
+        bar = -INFINITY;
+    }
+    __device__ __forceinline__ bool before(uint64_t k, int i) const { return key > k || (key == k && at < i); }
+    // Offers one candidate of every lane (those with `offer`); the whole warp takes part.
+    __device__ __forceinline__ void offer(bool offer, C value, int index, int top) {
+        const int lane = threadIdx.x & 31;
+        const uint64_t mine = offer ? order_key(value) : 0;
+        uint64_t bar_key = __shfl_sync(0xffffffffu, key, top - 1);
+        int bar_at = __shfl_sync(0xffffffffu, at, top - 1);
+        unsigned left = __ballot_sync(0xffffffffu, offer && (mine > bar_key || (mine == bar_key && index < bar_at)));
+        while (left) {
+            const int from = __ffs(left) - 1;
+            left &= left - 1;
+            const uint64_t k = __shfl_sync(0xffffffffu, mine, from);
+            const int i = __shfl_sync(0xffffffffu, index, from);
+            const int rank = __popc(__ballot_sync(0xffffffffu, before(k, i)));
+            const uint64_t up_key = __shfl_up_sync(0xffffffffu, key, 1);
+            const int up_at = __shfl_up_sync(0xffffffffu, at, 1);
+            if (lane > rank) {
+                key = up_key;
+                at = up_at;
+            } else if (lane == rank) {
+                key = k;
+                at = i;
             }
-            continue;
         }
-        LogSum<NP, C> sum;
-        sum.clear();
-        for (int64_t i = threadIdx.x; i < p.cols; i += blockDim.x) {
-            C z[NP];
-            load_logit<NP, T, C>(p, row, i, z);
-            sum.add(z);
-        }
-        for (int off = 16; off > 0; off >>= 1) {
-            LogSum<NP, C> o;
-            o.m = __shfl_xor_sync(0xffffffffu, sum.m, off);
-#pragma unroll
-            for (int k = 0; k < NP; ++k) {
-                o.S[k] = __shfl_xor_sync(0xffffffffu, sum.S[k], off);
-                o.T[k] = __shfl_xor_sync(0xffffffffu, sum.T[k], off);
+        bar_key = __shfl_sync(0xffffffffu, key, top - 1);
+        bar = value_of(bar_key);
+    }
+    // Merges another list of the same form (lane j offers its (j + 1)-th).
+    __device__ __forceinline__ void merge(uint64_t other_key, int other_at, int top) {
+        const int lane = threadIdx.x & 31;
+        for (int j = 0; j < top; ++j) {
+            const uint64_t k = __shfl_sync(0xffffffffu, other_key, j);
+            const int i = __shfl_sync(0xffffffffu, other_at, j);
+            const int rank = __popc(__ballot_sync(0xffffffffu, before(k, i)));
+            if (rank >= top) return;        // the other's list falls from here on
+            const uint64_t up_key = __shfl_up_sync(0xffffffffu, key, 1);
+            const int up_at = __shfl_up_sync(0xffffffffu, at, 1);
+            if (lane > rank) {
+                key = up_key;
+                at = up_at;
+            } else if (lane == rank) {
+                key = k;
+                at = i;
             }
-            sum.join(o);
         }
-        __syncthreads();
-        if (lane == 0) part[warp] = sum;
-        __syncthreads();
-        C L[NP];
-        sum = part[0];
-        for (int w = 1; w < warps; ++w) sum.join(part[w]);
-        if (sum.m != -INFINITY) {
-            s_log<NP, C>(sum.S, L);
+    }
+    static __device__ __forceinline__ C value_of(uint64_t k) {
+        if (k == 0) return -INFINITY;       // the list is not full
+        if (k == ~0ull) return NAN;
+        if constexpr (sizeof(C) == 4) {
+            const uint32_t b = static_cast<uint32_t>(k);
+            return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
         } else {
-#pragma unroll
-            for (int k = 0; k < NP; ++k) L[k] = C(0);
+            return __longlong_as_double(static_cast<long long>(k >> 63 ? k & 0x7fffffffffffffffull : ~k));
         }
-        if (threadIdx.x == 0) {
-            C z[NP], v[NP], H[NP];
-            const bool inside = token >= 0 && token < p.cols;
-            if (inside) {
-                load_logit<NP, T, C>(p, row, token, z);
-                log_prob<NP, C>(z, sum.m, L, v);
+    }
+};
+
+template <int NP, typename C>
+struct FwdShared {
+    RowSum<NP, C> part[16];
+    RowSum<NP, C> block;
+    uint64_t key[16][32];
+    int at[16][32];
+};
+
+// One pass over the logits: the blocks of a cluster (gridDim.x of them, one or more) share a row, each
+// thread keeps the running sums of its groups of 16 bytes per plane, and the parts are joined in the warp,
+// in the block and through distributed shared memory in the cluster's first block.  The next group's
+// loads are in flight while one is worked on.
+template <typename T, int NP>
+__global__ void __launch_bounds__(NP > 6 ? 256 : 512) token_log_probs_fwd_kernel(const __grid_constant__ LogProbParams p) {
+    using C = typename Compute<T>::type;
+    constexpr int VEC = lp_vec<T>();
+    __shared__ FwdShared<NP, C> sh;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int64_t row = blockIdx.y + static_cast<int64_t>(blockIdx.z) * gridDim.y;
+    if (row >= p.rows) return;               // the whole cluster
+    const int64_t token = p.tokens[row];
+    const bool first_block = blockIdx.x == 0;
+    if (token == p.ignore_index) {           // not read: zeros, and no alternatives
+        if (first_block) {
+            for (int i = threadIdx.x; i < p.np; i += blockDim.x) static_cast<C*>(p.logp[i])[row] = static_cast<C*>(p.entropy[i])[row] = C(0);
+            for (int i = threadIdx.x; i <= p.np; i += blockDim.x) static_cast<C*>(p.stats)[row * (p.np + 1) + i] = C(0);
+            for (int i = threadIdx.x; i < p.top; i += blockDim.x) {
+                p.top_tokens[row * p.top + i] = -1;
+                for (int k = 0; k < p.np; ++k) static_cast<C*>(p.top_logp[k])[row * p.top + i] = C(0);
             }
-            if (sum.m != -INFINITY) s_div<NP, C>(sum.T, sum.S, H);
-#pragma unroll
-            for (int k = 0; k < NP; ++k) {
-                if (k >= p.np) continue;
-                static_cast<C*>(p.logp[k])[row] = inside ? v[k] : C(NAN);
-                static_cast<C*>(p.entropy[k])[row] = sum.m != -INFINITY ? L[k] - H[k] : C(0);
-                static_cast<C*>(p.stats)[row * (p.np + 1) + 1 + k] = L[k];
-            }
-            static_cast<C*>(p.stats)[row * (p.np + 1)] = sum.m;
         }
-        // the alternatives, one pass each: the best logit below the last one in (value, index) order
-        uint64_t last_key = ~0ull;
-        int64_t last_at = -1;
-        for (int j = 0; j < p.top; ++j) {
-            uint64_t key = 0;
-            int64_t at = p.cols;
-            for (int64_t i = threadIdx.x; i < p.cols; i += blockDim.x) {
-                const uint64_t q = order_key(to_c<C>(static_cast<const T*>(p.x[0])[row * p.x_rs + i]));
-                if (j > 0 && (q > last_key || (q == last_key && i <= last_at))) continue;
-                if (at == p.cols || q > key) {
-                    key = q;
-                    at = i;
-                }
-            }
-            for (int off = 16; off > 0; off >>= 1) {
-                const uint64_t k2 = __shfl_xor_sync(0xffffffffu, key, off);
-                const int64_t a2 = __shfl_xor_sync(0xffffffffu, at, off);
-                if (a2 < p.cols && (at == p.cols || k2 > key || (k2 == key && a2 < at))) {
-                    key = k2;
-                    at = a2;
-                }
-            }
-            __syncthreads();
-            if (lane == 0) {
-                best_key[warp] = key;
-                best_at[warp] = at;
-            }
-            __syncthreads();
-            key = best_key[0];
-            at = best_at[0];
-            for (int w = 1; w < warps; ++w) {
-                const uint64_t k2 = best_key[w];
-                const int64_t a2 = best_at[w];
-                if (a2 < p.cols && (at == p.cols || k2 > key || (k2 == key && a2 < at))) {
-                    key = k2;
-                    at = a2;
-                }
-            }
-            last_key = key;
-            last_at = at;
-            if (threadIdx.x == 0) {
-                C z[NP], v[NP];
-                load_logit<NP, T, C>(p, row, at, z);
-                log_prob<NP, C>(z, sum.m, L, v);
-                p.top_tokens[row * p.top + j] = at;
+        return;                              // the whole cluster
+    }
+    const int64_t row_at = row * p.x_rs;
+    const bool aligned = p.aligned != 0;
+    RowGroups groups;
+    groups.set<T>(static_cast<const T*>(p.x[0]) + row_at, p.cols, aligned);
+    // this block's groups, and every thread of a warp the same number of steps
+    const int per_block = (groups.count + gridDim.x - 1) / gridDim.x;
+    const int begin = blockIdx.x * per_block, end = min(begin + per_block, groups.count);
+    const C scale = C(p.scale);
+    LogSum<NP, C> sum;
+    sum.clear();
+    Best<C> best;
+    best.clear();
+    Group<NP, T> now, next;
+    if (begin + static_cast<int>(threadIdx.x) < end) next.load(p, row_at, groups, begin + threadIdx.x, aligned);
+    for (int base = begin + warp * 32; base < end; base += blockDim.x) {
+        const int g = base + lane;
+        const bool live = g < end;
+        now = next;
+        if (g + static_cast<int>(blockDim.x) < end) next.load(p, row_at, groups, g + blockDim.x, aligned);
+        C top = -INFINITY;
+        if (live) {
 #pragma unroll
-                for (int k = 0; k < NP; ++k)
-                    if (k < p.np) static_cast<C*>(p.top_logp[k])[row * p.top + j] = v[k];
+            for (int i = 0; i < VEC / 2; ++i) {
+                C a, b;
+                now.v[0].get(i).get(a, b);
+                top = max_nan(top, max_nan(a, b));
             }
+            if (top * scale > sum.m) sum.raise(top * scale);
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) {
+                Two<C> u[NP];
+#pragma unroll
+                for (int k = 1; k < NP; ++k) u[k] = now.v[k].get(i);
+                if (scale != C(1)) {
+#pragma unroll
+                    for (int k = 1; k < NP; ++k) u[k] = u[k] * Two<C>(scale);
+                }
+                sum.add(now.v[0].get(i), scale, u);
+            }
+        }
+        if (p.top && __any_sync(0xffffffffu, live && !(top < best.bar))) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                C a, b;
+                now.v[0].get(i / 2).get(a, b);
+                const int index = g * VEC - groups.skew + i;
+                best.offer(live && index >= 0 && index < p.cols, i % 2 ? b : a, index, p.top);
+            }
+        }
+    }
+    RowSum<NP, C> all;
+    all.m = sum.m;
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+        C a, b;
+        sum.S[k].get(a, b);
+        all.S[k] = a + b;
+        sum.T[k].get(a, b);
+        all.T[k] = a + b;
+    }
+    all.join_warp();
+    if (lane == 0) sh.part[warp] = all;
+    if (p.top) {
+        sh.key[warp][lane] = best.key;
+        sh.at[warp][lane] = best.at;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        if (lane < warps) all = sh.part[lane];
+        else all.clear();
+        all.join_warp();
+        if (p.top)
+            for (int w = 1; w < warps; ++w) best.merge(sh.key[w][lane], sh.at[w][lane], p.top);
+    }
+    if (gridDim.x > 1) {
+        namespace cg = cooperative_groups;
+        cg::cluster_group cluster = cg::this_cluster();
+        if (warp == 0) {
+            if (lane == 0) sh.block = all;
+            if (p.top) {
+                sh.key[0][lane] = best.key;
+                sh.at[0][lane] = best.at;
+            }
+        }
+        cluster.sync();
+        if (first_block && warp == 0) {
+            if (lane < static_cast<int>(gridDim.x)) all = *cluster.map_shared_rank(&sh.block, lane);
+            else all.clear();
+            all.join_warp();
+            if (p.top)
+                for (unsigned o = 1; o < gridDim.x; ++o) {
+                    const FwdShared<NP, C>* other = cluster.map_shared_rank(&sh, o);
+                    best.merge(other->key[0][lane], other->at[0][lane], p.top);
+                }
+        }
+        cluster.sync();                      // the others' shared memory stays until it has been read
+    }
+    if (!first_block || warp != 0) return;
+    // the same in every lane: the normaliser's logarithm; then lane j writes alternative j, lane 0 the rest
+    C L[NP];
+    // a part with open logits has m > -inf; NaN sums without any (all NaN) count as open
+    const bool empty = all.m == -INFINITY && all.S[0] == C(0);
+    const C m = all.m == -INFINITY && !empty ? C(NAN) : all.m;
+    if (empty) {
+#pragma unroll
+        for (int k = 0; k < NP; ++k) L[k] = C(0);
+    } else {
+        s_log<NP, C>(all.S, L);
+    }
+    if (lane < p.top) {
+        C z[NP], v[NP];
+        load_logit<NP, T, C>(p, row, best.at, z);
+        log_prob<NP, C>(z, m, L, v);
+        p.top_tokens[row * p.top + lane] = best.at;
+#pragma unroll
+        for (int k = 0; k < NP; ++k)
+            if (k < p.np) static_cast<C*>(p.top_logp[k])[row * p.top + lane] = v[k];
+    }
+    if (lane == 0) {
+        C z[NP], v[NP], E[NP];
+        const bool inside = token >= 0 && token < p.cols;
+        if (inside) {
+            load_logit<NP, T, C>(p, row, token, z);
+            log_prob<NP, C>(z, m, L, v);
+        }
+        s_div<NP, C>(all.T, all.S, E);
+        C* stats = static_cast<C*>(p.stats) + row * (p.np + 1);
+        stats[0] = m;
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+            if (k >= p.np) continue;
+            static_cast<C*>(p.logp[k])[row] = inside ? v[k] : C(NAN);
+            static_cast<C*>(p.entropy[k])[row] = empty ? C(0) : L[k] - E[k];
+            stats[1 + k] = L[k];
         }
     }
 }
 
+// The gradient of a part of a row: blockIdx.x takes its share of the row's groups.  Everything that the row
+// has in common is folded into two series first: with d_i = logp_i,
+//   dx_i = p_i (*) (B (*) d_i + G) + scale (a [i = token] + sum_j c_j [i = top_j]),
+//   B = -scale b,  G = -scale (A + b (*) H).
+// The token and the alternatives are written again at the end, in full, by a thread each.
+template <int NP, typename C>
+struct RowGrad {
+    C m, L[NP], B[NP], G[NP];
+};
+
+template <int NP, typename T, typename C>
+__device__ __forceinline__ void grad_of(const RowGrad<NP, C>& r, bool has_b, const C (&z)[NP], C (&out)[NP]) {
+    C d[NP], P[NP], q[NP];
+    log_prob<NP, C>(z, r.m, r.L, d);
+    const C p0 = z[0] == -INFINITY ? C(0) : exp_small(d[0]);
+    s_exp_dir<NP, C>(d, P);
+#pragma unroll
+    for (int k = 0; k < NP; ++k) q[k] = r.G[k];
+    if (has_b) s_mul_acc<NP, C>(r.B, d, q);
+    s_mul<NP, C>(P, q, out);
+#pragma unroll
+    for (int k = 0; k < NP; ++k) out[k] = p0 == C(0) ? C(0) : p0 * out[k];
+}
+
 template <typename T, int NP>
-__global__ void __launch_bounds__(256) token_log_probs_bwd_kernel(const LogProbParams p) {
+__global__ void __launch_bounds__(256) token_log_probs_bwd_kernel(const __grid_constant__ LogProbParams p) {
     using C = typename Compute<T>::type;
+    constexpr int VEC = lp_vec<T>();
+    const int64_t row = blockIdx.y + static_cast<int64_t>(blockIdx.z) * gridDim.y;
+    if (row >= p.rows) return;
+    const int64_t token = p.tokens[row], x_at = row * p.x_rs, dx_at = row * p.dx_rs;
+    const C* stats = static_cast<const C*>(p.stats_in) + row * (p.np + 1);
     const C scale = C(p.scale);
-    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        const int64_t token = p.tokens[row];
-        const C m = static_cast<const C*>(p.stats_in)[row * (p.np + 1)];
-        if (token == p.ignore_index || m == -INFINITY) {
-            for (int64_t i = threadIdx.x; i < p.cols; i += blockDim.x)
-                for (int k = 0; k < p.np; ++k) static_cast<T*>(p.dx[k])[row * p.dx_rs + i] = from_c<T>(C(0));
-            continue;
-        }
-        C L[NP], a[NP], b[NP], A[NP], H[NP], z[NP];
+    RowGrad<NP, C> r;
+    r.m = stats[0];
+    const bool dead = token == p.ignore_index || r.m == -INFINITY;      // no gradient at all
+    RowGroups groups;
+    const T* row0 = static_cast<const T*>(p.x[0]) + x_at;
+    bool aligned = p.aligned != 0;
+    if (aligned && reinterpret_cast<uintptr_t>(row0) % 16 != reinterpret_cast<uintptr_t>(static_cast<const T*>(p.dx[0]) + dx_at) % 16)
+        aligned = false;                                                // the two rows start apart
+    groups.set<T>(row0, p.cols, aligned);
+    const int per_block = (groups.count + gridDim.x - 1) / gridDim.x;
+    const int begin = blockIdx.x * per_block, end = min(begin + per_block, groups.count);
+    C a[NP];
+#pragma unroll
+    for (int k = 0; k < NP; ++k) a[k] = r.L[k] = r.B[k] = r.G[k] = C(0);
+    if (!dead) {
+        C A[NP], b[NP], H[NP], z[NP];
         const bool inside = token >= 0 && token < p.cols;
         bool open = false;
-        if (inside && p.has_a) {
-            load_logit<NP, T, C>(p, row, token, z);
-            open = z[0] != -INFINITY;
-        }
+        if (inside && p.has_a) open = to_c<C>(row0[token]) * scale != -INFINITY;
 #pragma unroll
         for (int k = 0; k < NP; ++k) {
             const bool live = k < p.np;
-            L[k] = live ? static_cast<const C*>(p.stats_in)[row * (p.np + 1) + 1 + k] : C(0);
+            r.L[k] = live ? stats[1 + k] : C(0);
             H[k] = live ? static_cast<const C*>(p.h[k])[row] : C(0);
             a[k] = !live || !p.has_a ? C(0) : !inside ? C(NAN) : open ? static_cast<const C*>(p.ga[k])[row] : C(0);
             b[k] = live && p.has_b ? static_cast<const C*>(p.gb[k])[row] : C(0);
             A[k] = a[k];
         }
         for (int j = 0; j < (p.has_c ? p.top : 0); ++j) {
-            load_logit<NP, T, C>(p, row, p.top_at[row * p.top + j], z);
-            if (z[0] == -INFINITY) continue;
+            if (to_c<C>(row0[p.top_at[row * p.top + j]]) * scale == -INFINITY) continue;
 #pragma unroll
             for (int k = 0; k < NP; ++k)
                 if (k < p.np) A[k] += static_cast<const C*>(p.gc[k])[row * p.top + j];
         }
-        for (int64_t i = threadIdx.x; i < p.cols; i += blockDim.x) {
-            C lp[NP], P[NP], q[NP], r[NP];
-            load_logit<NP, T, C>(p, row, i, z);
-            const bool masked = z[0] == -INFINITY;
-            log_prob<NP, C>(z, m, L, lp);
-            s_exp<NP, C>(lp, P);
-            if (P[0] == C(0)) {
+        if (p.has_b) s_mul_acc<NP, C>(b, H, A);
 #pragma unroll
-                for (int k = 0; k < NP; ++k) r[k] = C(0);
-            } else {
-#pragma unroll
-                for (int k = 0; k < NP; ++k) {
-                    lp[k] += H[k];
-                    q[k] = A[k];
-                }
-                s_mul_acc<NP, C>(b, lp, q);
-                s_mul<NP, C>(P, q, r);
-#pragma unroll
-                for (int k = 0; k < NP; ++k) r[k] = -r[k];
-            }
-            if (!masked) {
-                if (i == token) {
-#pragma unroll
-                    for (int k = 0; k < NP; ++k) r[k] += a[k];
-                }
-                for (int j = 0; j < (p.has_c ? p.top : 0); ++j)
-                    if (p.top_at[row * p.top + j] == i) {
-#pragma unroll
-                        for (int k = 0; k < NP; ++k)
-                            if (k < p.np) r[k] += static_cast<const C*>(p.gc[k])[row * p.top + j];
-                    }
-            }
-#pragma unroll
-            for (int k = 0; k < NP; ++k)
-                if (k < p.np) static_cast<T*>(p.dx[k])[row * p.dx_rs + i] = from_c<T>(r[k] * scale);
+        for (int k = 0; k < NP; ++k) {
+            r.G[k] = -scale * A[k];
+            r.B[k] = -scale * b[k];
         }
     }
+    Two<C> L[NP], B[NP], G[NP];
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+        L[k] = Two<C>(-r.L[k]);
+        B[k] = Two<C>(r.B[k]);
+        G[k] = Two<C>(r.G[k]);
+    }
+    for (int g = begin + threadIdx.x; g < end; g += blockDim.x) {
+        Group<NP, T> x;
+        if (!dead) x.load(p, x_at, groups, g, aligned);
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) {
+            Two<C> d[NP], e[NP], q[NP], o[NP];
+            if (dead) {
+#pragma unroll
+                for (int k = 0; k < NP; ++k) x.v[k].set(i, Two<C>(C(0)));
+                continue;
+            }
+            d[0] = fma2(x.v[0].get(i), Two<C>(scale), Two<C>(-r.m)) + L[0];
+#pragma unroll
+            for (int k = 1; k < NP; ++k) d[k] = fma2(x.v[k].get(i), Two<C>(scale), L[k]);
+            C d0, d1;
+            d[0].get(d0, d1);
+            const C p0 = exp_small(d0), p1 = exp_small(d1);
+            e[0] = Two<C>(C(1));
+#pragma unroll
+            for (int k = 1; k < NP; ++k) {
+                Two<C> t = d[k];
+#pragma unroll
+                for (int j = 1; j < k; ++j) t = fma2(d[j] * e[k - j], Two<C>(C(j) / C(k)), t);
+                e[k] = t;
+            }
+#pragma unroll
+            for (int k = 0; k < NP; ++k) q[k] = G[k];
+            if (p.has_b) pair_mul_acc<NP, C>(B, d, q);
+            pair_mul<NP, C>(e, q, o);
+            const Two<C> w(p0, p1);
+#pragma unroll
+            for (int k = 0; k < NP; ++k) o[k] = o[k] * w;
+            if (p0 == C(0) || p1 == C(0)) {      // masked: 0 whatever the directions hold
+#pragma unroll
+                for (int k = 0; k < NP; ++k) {
+                    C u, v;
+                    o[k].get(u, v);
+                    o[k] = Two<C>(p0 == C(0) ? C(0) : u, p1 == C(0) ? C(0) : v);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < NP; ++k) x.v[k].set(i, o[k]);
+        }
+        const int64_t first = static_cast<int64_t>(g) * VEC - groups.skew;
+        if (aligned && first >= 0 && first + VEC <= p.cols) {
+#pragma unroll
+            for (int k = 0; k < NP; ++k)
+                if (NP <= 6 || k < p.np) *reinterpret_cast<Raw<T, VEC>*>(static_cast<T*>(p.dx[k]) + dx_at + first) = x.v[k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < NP; ++k) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (first + j >= 0 && first + j < p.cols && (NP <= 6 || k < p.np)) {
+                        const uint64_t bits = x.v[k].bits(j);
+                        memcpy(static_cast<T*>(p.dx[k]) + dx_at + first + j, &bits, sizeof(T));
+                    }
+            }
+        }
+    }
+    if (dead) return;
+    __syncthreads();
+    const int specials = 1 + (p.has_c ? p.top : 0);
+    if (static_cast<int>(threadIdx.x) >= specials) return;
+    const int64_t at = threadIdx.x == 0 ? token : p.top_at[row * p.top + threadIdx.x - 1];
+    const int64_t low = static_cast<int64_t>(begin) * VEC - groups.skew, high = static_cast<int64_t>(end) * VEC - groups.skew;
+    if (at < 0 || at >= p.cols || at < low || at >= high) return;
+    C z[NP], o[NP];
+    load_logit<NP, T, C>(p, row, at, z);
+    if (z[0] == -INFINITY) return;               // masked: the 0 stands
+    grad_of<NP, T, C>(r, p.has_b != 0, z, o);
+    if (at == token) {
+#pragma unroll
+        for (int k = 0; k < NP; ++k) o[k] += scale * a[k];
+    }
+    for (int j = 0; j < (p.has_c ? p.top : 0); ++j)
+        if (p.top_at[row * p.top + j] == at) {
+#pragma unroll
+            for (int k = 0; k < NP; ++k)
+                if (k < p.np) o[k] += scale * static_cast<const C*>(p.gc[k])[row * p.top + j];
+        }
+#pragma unroll
+    for (int k = 0; k < NP; ++k)
+        if (k < p.np) static_cast<T*>(p.dx[k])[dx_at + at] = from_c<T>(o[k]);
+}
+
+// Rows over the grid's y and z (65535 blocks at most along each).
+static dim3 row_grid(int64_t rows, int64_t per_row) {
+    const int64_t y = std::min<int64_t>(rows, 65535);
+    return dim3(static_cast<unsigned>(per_row), static_cast<unsigned>(y), static_cast<unsigned>(ceil_div(rows, y)));
 }
 
 template <typename T, int NP>
-static void launch_log_probs(const LogProbParams& p, bool backward, cudaStream_t s) {
-    const int grid = static_cast<int>(std::min<int64_t>(p.rows, static_cast<int64_t>(num_sms()) * 16));
-    if (backward) PK_LAUNCHED(token_log_probs_bwd_kernel<T, NP><<<grid, 256, 0, s>>>(p));
-    else PK_LAUNCHED(token_log_probs_fwd_kernel<T, NP><<<grid, 256, 0, s>>>(p));
+static cudaError_t launch_log_probs(const LogProbParams& p, bool backward, cudaStream_t s) {
+    const int64_t groups = ceil_div(p.cols, lp_vec<T>()) + 1;
+    if (backward) {
+        // about four groups a thread; a row that is shorter than that takes one block
+        const int64_t threads = groups >= 256 ? 256 : 128;
+        const int64_t per_row = std::max<int64_t>(1, groups / (4 * threads));
+        PK_LAUNCHED(token_log_probs_bwd_kernel<T, NP><<<row_grid(p.rows, per_row), static_cast<int>(threads), 0, s>>>(p));
+        return cudaSuccess;
+    }
+    // a row is shared by more blocks while the blocks do not fill the GPU and each keeps a group a thread
+    const int threads = groups >= 2048 && NP <= 6 ? 512 : groups >= 512 ? 256 : 128;
+    int share = 1;
+    while (share < 8 && p.rows * share < num_sms() && groups / (2 * share) >= threads) share *= 2;
+    cudaLaunchConfig_t config{};
+    config.gridDim = row_grid(p.rows, share);
+    config.blockDim = dim3(threads);
+    config.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = share;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    config.attrs = &attr;
+    config.numAttrs = share > 1 ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&config, token_log_probs_fwd_kernel<T, NP>, p);
+    note_launch();
+    return e;
 }
 
 template <typename T>
-static void launch_log_probs_np(const LogProbParams& p, bool backward, cudaStream_t s) {
+static cudaError_t launch_log_probs_np(const LogProbParams& p, bool backward, cudaStream_t s) {
     switch (p.np) {
-        case 1: launch_log_probs<T, 1>(p, backward, s); break;
-        case 2: launch_log_probs<T, 2>(p, backward, s); break;
-        case 3: launch_log_probs<T, 3>(p, backward, s); break;
-        case 4: launch_log_probs<T, 4>(p, backward, s); break;
-        case 5: launch_log_probs<T, 5>(p, backward, s); break;
-        case 6: launch_log_probs<T, 6>(p, backward, s); break;
-        case 7: case 8: case 9: launch_log_probs<T, 9>(p, backward, s); break;
-        default: launch_log_probs<T, 16>(p, backward, s); break;
+        case 1: return launch_log_probs<T, 1>(p, backward, s);
+        case 2: return launch_log_probs<T, 2>(p, backward, s);
+        case 3: return launch_log_probs<T, 3>(p, backward, s);
+        case 4: return launch_log_probs<T, 4>(p, backward, s);
+        case 5: return launch_log_probs<T, 5>(p, backward, s);
+        case 6: return launch_log_probs<T, 6>(p, backward, s);
+        case 7: case 8: case 9: return launch_log_probs<T, 9>(p, backward, s);
+        default: return launch_log_probs<T, 16>(p, backward, s);
     }
 }
 
-static int run_log_probs(int dtype, const LogProbParams& p, bool backward, void* stream, const char* name) {
+static int run_log_probs(int dtype, LogProbParams& p, bool backward, void* stream, const char* name) {
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    // whole groups are aligned in every plane when all bases lie alike within 16 bytes
+    p.aligned = 1;
+    for (int k = 1; k < p.np; ++k)
+        if (reinterpret_cast<uintptr_t>(p.x[k]) % 16 != reinterpret_cast<uintptr_t>(p.x[0]) % 16 ||
+            (backward && reinterpret_cast<uintptr_t>(p.dx[k]) % 16 != reinterpret_cast<uintptr_t>(p.dx[0]) % 16))
+            p.aligned = 0;
     void* tok;
+    cudaError_t e = cudaSuccess;
     prof_begin(name, s, &tok);
     switch (dtype) {
-        case PK_F32: launch_log_probs_np<float>(p, backward, s); break;
-        case PK_F64: launch_log_probs_np<double>(p, backward, s); break;
-        case PK_BF16: launch_log_probs_np<__nv_bfloat16>(p, backward, s); break;
-        default: launch_log_probs_np<__half>(p, backward, s); break;
+        case PK_F32: e = launch_log_probs_np<float>(p, backward, s); break;
+        case PK_F64: e = launch_log_probs_np<double>(p, backward, s); break;
+        case PK_BF16: e = launch_log_probs_np<__nv_bfloat16>(p, backward, s); break;
+        default: e = launch_log_probs_np<__half>(p, backward, s); break;
     }
     prof_end(name, s, tok);
+    if (e != cudaSuccess) return cuda_fail(e, name);
     PK_CHECK_LAUNCH(name);
     return PK_OK;
 }
@@ -372,7 +735,7 @@ static int check_log_probs(int dtype, int degree, int64_t rows, int64_t cols, in
     if (dtype != PK_F32 && dtype != PK_F64 && dtype != PK_BF16 && dtype != PK_F16)
         return fail(PK_ERR_UNSUPPORTED, what + ": unsupported dtype");
     if (degree < 0 || degree >= PK_MAX_PLANES) return fail(PK_ERR_UNSUPPORTED, what + ": degree out of range");
-    if (rows < 0 || cols < 1 || cols > 0x7fffffff) return fail(PK_ERR_ARG, what + ": bad extent");
+    if (rows < 0 || cols < 1 || cols > 0x7fffff00) return fail(PK_ERR_ARG, what + ": bad extent");
     if (top < 0 || top > LP_MAX_TOP || top > cols) return fail(PK_ERR_ARG, what + ": bad number of alternatives");
     if (rows == 0) return PK_OK;
     if (!x || !tokens || !stats || (top && !top_tokens)) return fail(PK_ERR_ARG, what + ": null pointer");

@@ -148,9 +148,6 @@ struct alignas(sizeof(T) * V) Raw {
     }
 };
 
-template <typename C>
-__device__ __forceinline__ Two<C> operator-(Two<C> a, Two<C> b) { return fma2(b, Two<C>(C(-1)), a); }
-
 // 32-bit division by a divisor known at launch: q = (t + (n - t) / 2) >> (l - 1) with t = high(m n),
 // 2^(l-1) < d <= 2^l, m = floor(2^32 (2^l - d) / d) + 1 (Granlund and Montgomery, "Division by invariant
 // integers using multiplication", PLDI 1994).
