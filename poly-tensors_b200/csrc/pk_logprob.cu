@@ -1,9 +1,9 @@
 // Log probabilities of given tokens, entropy and top alternatives of a row of logits, and their
 // gradient.  A row has V logits x of n+1 planes; z = scale * x (scale = 1 / temperature), (*) is the
-// truncated series product.  With m = max z_0 and w_i = exp(z_i - m) (a series):
+// truncated series product.  With m near max z_0 and w_i = exp(z_i - m) (a series):
 //   S = sum_i w_i,  L = log S,  logp_i = (z_i - m) - L,  H = L - (sum_i w_i (*) (z_i - m)) / S.
-// L lies in [0, log V] and both terms of H are nonnegative at plane 0, so nothing cancels however large
-// the logits are.  Backward, with p_i = exp(logp_i), upstream series a (token), b (entropy), c_j
+// At plane 0, L and the mean of z - m are of the size of log V, so nothing cancels however large the
+// logits are.  Backward, with p_i = exp(logp_i), upstream series a (token), b (entropy), c_j
 // (alternative j) and A = a + sum_j c_j:
 //   dx_i = scale ( a [i = token] + sum_j c_j [i = top_j] - p_i (*) (A + b (*) (logp_i + H)) ).
 // A logit whose constant plane is -inf is masked: it takes no part whatever its other planes hold, its
@@ -77,12 +77,16 @@ constexpr int lp_vec() { return 16 / sizeof(T); }
 // 16-byte boundary at or before the row, so that whole groups are aligned whatever the row's offset.
 struct RowGroups {
     int skew, count;
+    int full, last;          // groups full .. last - 1 lie within the row and are aligned
     template <typename T>
     __device__ __forceinline__ void set(const void* row, int64_t cols, bool aligned) {
         constexpr int VEC = lp_vec<T>();
         skew = aligned ? static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T)) : 0;
         count = static_cast<int>((cols + skew + VEC - 1) / VEC);
+        full = skew ? 1 : 0;
+        last = aligned ? static_cast<int>((cols + skew) / VEC) : 0;
     }
+    __device__ __forceinline__ bool whole(int g) const { return g >= full && g < last; }
 };
 
 // One group of every plane; elements outside the row read as masked (-inf, no direction).
@@ -91,9 +95,9 @@ struct Group {
     static constexpr int VEC = lp_vec<T>();
     Raw<T, VEC> v[NP];
 
-    __device__ __forceinline__ void load(const LogProbParams& p, int64_t row_at, const RowGroups& row, int g, bool aligned) {
+    __device__ __forceinline__ void load(const LogProbParams& p, int64_t row_at, const RowGroups& row, int g) {
         const int64_t first = static_cast<int64_t>(g) * VEC - row.skew;
-        if (aligned && first >= 0 && first + VEC <= p.cols) {
+        if (row.whole(g)) {
 #pragma unroll
             for (int k = 0; k < NP; ++k) {
                 if constexpr (NP > 6) v[k] = Raw<T, VEC>{};
@@ -121,8 +125,14 @@ struct Group {
 template <typename C>
 __device__ __forceinline__ C nan_or_zero(C v) { return v == v ? C(0) : v; }
 
-// Running state of a part of a row: the largest z_0 seen, S and T = sum w (*) (z - m) below it.  Two sums
-// of each run side by side (even and odd elements) and are joined at the end.
+// How far a logit may lie above a thread's m before the sums are rescaled.  m is the largest logit of the
+// thread's first group and nearly always stays: weights reach e^8, which costs T / S (at most 8 at plane 0)
+// no digits that matter and saves a rescaling in most early steps of every warp.
+constexpr int LP_SLACK = 8;
+
+// Running state of a part of a row below a reference m (its first largest z_0): S = sum w and
+// T = sum w (*) (z - m), w = exp(z - m).  Two sums of each run side by side (even and odd elements) and are
+// joined at the end.
 template <int NP, typename C>
 struct LogSum {
     C m;
@@ -132,7 +142,7 @@ struct LogSum {
 #pragma unroll
         for (int k = 0; k < NP; ++k) S[k] = T[k] = Two<C>(C(0));
     }
-    // The same sums below a larger maximum.
+    // The same sums below a larger m.
     __device__ __forceinline__ void raise(C to) {
         const C d = m - to, f = m == -INFINITY ? C(0) : exp_fast(d);
         if (f == C(0)) {
@@ -263,8 +273,21 @@ struct Best {
         bar = -INFINITY;
     }
     __device__ __forceinline__ bool before(uint64_t k, int i) const { return key > k || (key == k && at < i); }
+    // A first bar from each lane's largest logit: `top` of the 32 are no smaller than the top-th of them.
+    __device__ __forceinline__ void start(C lane_top, int top) {
+        const uint64_t mine = order_key(lane_top);
+        int rank = 0;
+        for (int j = 0; j < 32; ++j) {
+            const uint64_t k = __shfl_sync(0xffffffffu, mine, j);
+            rank += k > mine || (k == mine && j < static_cast<int>(threadIdx.x & 31));
+        }
+        const unsigned at_bar = __ballot_sync(0xffffffffu, rank == top - 1);
+        bar = __shfl_sync(0xffffffffu, lane_top, __ffs(at_bar) - 1);
+    }
     // Offers one candidate of every lane (those with `offer`); the whole warp takes part.
     __device__ __forceinline__ void offer(bool offer, C value, int index, int top) {
+        offer = offer && !(value < bar);
+        if (!__any_sync(0xffffffffu, offer)) return;
         const int lane = threadIdx.x & 31;
         const uint64_t mine = offer ? order_key(value) : 0;
         uint64_t bar_key = __shfl_sync(0xffffffffu, key, top - 1);
@@ -287,7 +310,7 @@ struct Best {
             }
         }
         bar_key = __shfl_sync(0xffffffffu, key, top - 1);
-        bar = value_of(bar_key);
+        if (bar_key != 0) bar = max_nan(bar, value_of(bar_key));
     }
     // Merges another list of the same form (lane j offers its (j + 1)-th).
     __device__ __forceinline__ void merge(uint64_t other_key, int other_at, int top) {
@@ -309,7 +332,6 @@ struct Best {
         }
     }
     static __device__ __forceinline__ C value_of(uint64_t k) {
-        if (k == 0) return -INFINITY;       // the list is not full
         if (k == ~0ull) return NAN;
         if constexpr (sizeof(C) == 4) {
             const uint32_t b = static_cast<uint32_t>(k);
@@ -328,21 +350,39 @@ struct FwdShared {
     int at[16][32];
 };
 
+// Groups of a thread that are in flight while as many are worked on: enough bytes to cover the latency of
+// memory at low degrees, what the registers allow at high ones.
+template <int NP>
+constexpr int lp_depth() { return NP == 1 ? 2 : 1; }
+
 // One pass over the logits: the blocks of a cluster (gridDim.x of them, one or more) share a row, each
 // thread keeps the running sums of its groups of 16 bytes per plane, and the parts are joined in the warp,
-// in the block and through distributed shared memory in the cluster's first block.  The next group's
-// loads are in flight while one is worked on.
+// in the block and through distributed shared memory in the cluster's first block.
 template <typename T, int NP>
 __global__ void __launch_bounds__(NP > 6 ? 256 : 512) token_log_probs_fwd_kernel(const __grid_constant__ LogProbParams p) {
     using C = typename Compute<T>::type;
-    constexpr int VEC = lp_vec<T>();
+    constexpr int VEC = lp_vec<T>(), DEPTH = lp_depth<NP>();
     __shared__ FwdShared<NP, C> sh;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int64_t row = blockIdx.y + static_cast<int64_t>(blockIdx.z) * gridDim.y;
     if (row >= p.rows) return;               // the whole cluster
+    const int64_t row_at = row * p.x_rs;
+    const bool aligned = p.aligned != 0;
+    RowGroups groups;
+    groups.set<T>(static_cast<const T*>(p.x[0]) + row_at, p.cols, aligned);
+    // this block's groups, and every thread of a warp the same number of steps
+    const int per_block = (groups.count + gridDim.x - 1) / gridDim.x;
+    const int begin = blockIdx.x * per_block, end = min(begin + per_block, groups.count);
+    const int stride = blockDim.x;
+    Group<NP, T> now[DEPTH], next[DEPTH];
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+        const int g = begin + static_cast<int>(threadIdx.x) + d * stride;
+        if (g < end) next[d].load(p, row_at, groups, g);
+    }
     const int64_t token = p.tokens[row];
     const bool first_block = blockIdx.x == 0;
-    if (token == p.ignore_index) {           // not read: zeros, and no alternatives
+    if (token == p.ignore_index) {           // zeros, and no alternatives
         if (first_block) {
             for (int i = threadIdx.x; i < p.np; i += blockDim.x) static_cast<C*>(p.logp[i])[row] = static_cast<C*>(p.entropy[i])[row] = C(0);
             for (int i = threadIdx.x; i <= p.np; i += blockDim.x) static_cast<C*>(p.stats)[row * (p.np + 1) + i] = C(0);
@@ -353,53 +393,66 @@ __global__ void __launch_bounds__(NP > 6 ? 256 : 512) token_log_probs_fwd_kernel
         }
         return;                              // the whole cluster
     }
-    const int64_t row_at = row * p.x_rs;
-    const bool aligned = p.aligned != 0;
-    RowGroups groups;
-    groups.set<T>(static_cast<const T*>(p.x[0]) + row_at, p.cols, aligned);
-    // this block's groups, and every thread of a warp the same number of steps
-    const int per_block = (groups.count + gridDim.x - 1) / gridDim.x;
-    const int begin = blockIdx.x * per_block, end = min(begin + per_block, groups.count);
+    const bool inside = token >= 0 && token < p.cols;
+    C chosen[NP];                            // the token's logit, asked for now, used at the end
+    if (first_block && threadIdx.x == 0 && inside) load_logit<NP, T, C>(p, row, token, chosen);
     const C scale = C(p.scale);
     LogSum<NP, C> sum;
     sum.clear();
     Best<C> best;
     best.clear();
-    Group<NP, T> now, next;
-    if (begin + static_cast<int>(threadIdx.x) < end) next.load(p, row_at, groups, begin + threadIdx.x, aligned);
-    for (int base = begin + warp * 32; base < end; base += blockDim.x) {
-        const int g = base + lane;
-        const bool live = g < end;
-        now = next;
-        if (g + static_cast<int>(blockDim.x) < end) next.load(p, row_at, groups, g + blockDim.x, aligned);
-        C top = -INFINITY;
-        if (live) {
+    for (int base = begin + warp * 32; base < end; base += DEPTH * stride) {
 #pragma unroll
-            for (int i = 0; i < VEC / 2; ++i) {
-                C a, b;
-                now.v[0].get(i).get(a, b);
-                top = max_nan(top, max_nan(a, b));
-            }
-            if (top * scale > sum.m) sum.raise(top * scale);
+        for (int d = 0; d < DEPTH; ++d) now[d] = next[d];
 #pragma unroll
-            for (int i = 0; i < VEC / 2; ++i) {
-                Two<C> u[NP];
-#pragma unroll
-                for (int k = 1; k < NP; ++k) u[k] = now.v[k].get(i);
-                if (scale != C(1)) {
-#pragma unroll
-                    for (int k = 1; k < NP; ++k) u[k] = u[k] * Two<C>(scale);
-                }
-                sum.add(now.v[0].get(i), scale, u);
-            }
+        for (int d = 0; d < DEPTH; ++d) {
+            const int g = base + lane + (DEPTH + d) * stride;
+            if (g < end) next[d].load(p, row_at, groups, g);
         }
-        if (p.top && __any_sync(0xffffffffu, live && !(top < best.bar))) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                C a, b;
-                now.v[0].get(i / 2).get(a, b);
-                const int index = g * VEC - groups.skew + i;
-                best.offer(live && index >= 0 && index < p.cols, i % 2 ? b : a, index, p.top);
+        for (int d = 0; d < DEPTH; ++d) {
+            const int g = base + lane + d * stride;
+            const bool live = g < end;
+            C top = -INFINITY;
+            if (live) {
+#pragma unroll
+                for (int i = 0; i < VEC / 2; ++i) {
+                    C a, b;
+                    now[d].v[0].get(i).get(a, b);
+                    top = max_nan(top, max_nan(a, b));
+                }
+                if (top * scale > sum.m + C(LP_SLACK)) sum.raise(top * scale);
+#pragma unroll
+                for (int i = 0; i < VEC / 2; ++i) {
+                    Two<C> u[NP];
+#pragma unroll
+                    for (int k = 1; k < NP; ++k) u[k] = now[d].v[k].get(i);
+                    if (scale != C(1)) {
+#pragma unroll
+                        for (int k = 1; k < NP; ++k) u[k] = u[k] * Two<C>(scale);
+                    }
+                    sum.add(now[d].v[0].get(i), scale, u);
+                }
+            }
+            if (p.top) {
+                if (d == 0 && base == begin + warp * 32) best.start(top, p.top);
+                if (__any_sync(0xffffffffu, live && !(top < best.bar))) {
+                    unsigned open = 0;
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        C a, b;
+                        now[d].v[0].get(i / 2).get(a, b);
+                        const int index = g * VEC - groups.skew + i;
+                        open |= (live && index >= 0 && index < p.cols && !((i % 2 ? b : a) < best.bar) ? 1u : 0u) << i;
+                    }
+                    // rare: the values are read again, so that this stays one short loop
+                    while (__any_sync(0xffffffffu, open != 0)) {
+                        const int index = g * VEC - groups.skew + __ffs(open) - 1;
+                        const C value = open ? to_c<C>(static_cast<const T*>(p.x[0])[row_at + index]) : C(0);
+                        best.offer(open != 0, value, index, p.top);
+                        open &= open - 1;
+                    }
+                }
             }
         }
     }
@@ -472,12 +525,8 @@ __global__ void __launch_bounds__(NP > 6 ? 256 : 512) token_log_probs_fwd_kernel
             if (k < p.np) static_cast<C*>(p.top_logp[k])[row * p.top + lane] = v[k];
     }
     if (lane == 0) {
-        C z[NP], v[NP], E[NP];
-        const bool inside = token >= 0 && token < p.cols;
-        if (inside) {
-            load_logit<NP, T, C>(p, row, token, z);
-            log_prob<NP, C>(z, m, L, v);
-        }
+        C v[NP], E[NP];
+        if (inside) log_prob<NP, C>(chosen, m, L, v);
         s_div<NP, C>(all.T, all.S, E);
         C* stats = static_cast<C*>(p.stats) + row * (p.np + 1);
         stats[0] = m;
@@ -574,7 +623,7 @@ __global__ void __launch_bounds__(256) token_log_probs_bwd_kernel(const __grid_c
     }
     for (int g = begin + threadIdx.x; g < end; g += blockDim.x) {
         Group<NP, T> x;
-        if (!dead) x.load(p, x_at, groups, g, aligned);
+        if (!dead) x.load(p, x_at, groups, g);
 #pragma unroll
         for (int i = 0; i < VEC / 2; ++i) {
             Two<C> d[NP], e[NP], q[NP], o[NP];
@@ -616,7 +665,7 @@ __global__ void __launch_bounds__(256) token_log_probs_bwd_kernel(const __grid_c
             for (int k = 0; k < NP; ++k) x.v[k].set(i, o[k]);
         }
         const int64_t first = static_cast<int64_t>(g) * VEC - groups.skew;
-        if (aligned && first >= 0 && first + VEC <= p.cols) {
+        if (groups.whole(g)) {
 #pragma unroll
             for (int k = 0; k < NP; ++k)
                 if (NP <= 6 || k < p.np) *reinterpret_cast<Raw<T, VEC>*>(static_cast<T*>(p.dx[k]) + dx_at + first) = x.v[k];
@@ -675,9 +724,9 @@ static cudaError_t launch_log_probs(const LogProbParams& p, bool backward, cudaS
         return cudaSuccess;
     }
     // a row is shared by more blocks while the blocks do not fill the GPU and each keeps a group a thread
-    const int threads = groups >= 2048 && NP <= 6 ? 512 : groups >= 512 ? 256 : 128;
     int share = 1;
-    while (share < 8 && p.rows * share < num_sms() && groups / (2 * share) >= threads) share *= 2;
+    while (share < 8 && p.rows * share < num_sms() && groups / (2 * share) >= 256) share *= 2;
+    const int threads = share > 1 && groups / share >= 1024 && NP <= 6 ? 512 : groups >= 512 ? 256 : 128;
     cudaLaunchConfig_t config{};
     config.gridDim = row_grid(p.rows, share);
     config.blockDim = dim3(threads);
