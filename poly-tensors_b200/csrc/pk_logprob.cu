@@ -44,7 +44,8 @@ struct LogProbParams {
     const void* stats_in;
 };
 
-constexpr int LP_MAX_TOP = 32;
+constexpr int LP_MAX_TOP = 32;       // a warp's lanes
+constexpr int LP_MAX_SHARE = 8;      // blocks of a row's cluster (the portable limit)
 
 __device__ __forceinline__ float exp_fast(float x) {
     // 2^(x log2 e) in hardware: the argument's rounding, |x| 2^-24, is the same size as the logit's own
@@ -249,105 +250,115 @@ __device__ __forceinline__ void log_prob(const C (&z)[NP], C m, const C (&L)[NP]
     for (int k = 1; k < NP; ++k) out[k] = masked ? C(0) : z[k] - L[k];
 }
 
-// A value as an unsigned integer in the same order, NaN above everything, -0 as +0.
-__device__ __forceinline__ uint64_t order_key(float v) {
-    if (v != v) return ~0ull;
-    const uint32_t b = __float_as_uint(v + 0.0f);
-    return b & 0x80000000u ? static_cast<uint32_t>(~b) : static_cast<uint64_t>(b | 0x80000000u);
-}
-__device__ __forceinline__ uint64_t order_key(double v) {
-    if (v != v) return ~0ull;
-    const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v + 0.0));
-    return b >> 63 ? ~b : b | (1ull << 63);
-}
-
-// A warp's best logits so far: lane j holds the (j + 1)-th in (value falling, index rising) order.
-template <typename C>
-struct Best {
-    uint64_t key;
-    int at;
-    C bar;          // a value below this cannot enter the first `top`
-    __device__ __forceinline__ void clear() {
-        key = 0;
-        at = 0x7fffffff;
-        bar = -INFINITY;
+// A logit and its index as one key: a larger key is a larger logit, or the same with a lower index.  NaN
+// stands above every number, -0 with +0; the all-zero key is below every logit.
+template <typename C> struct Key;
+template <> struct Key<float> {
+    uint64_t k;
+    __device__ __forceinline__ static Key make(float v, int at) {
+        const uint32_t b = __float_as_uint(v + 0.0f);
+        const uint32_t o = v != v ? 0xffffffffu : b & 0x80000000u ? ~b : b | 0x80000000u;
+        return {static_cast<uint64_t>(o) << 32 | ~static_cast<uint32_t>(at)};
     }
-    __device__ __forceinline__ bool before(uint64_t k, int i) const { return key > k || (key == k && at < i); }
-    // A first bar from each lane's largest logit: `top` of the 32 are no smaller than the top-th of them.
-    __device__ __forceinline__ void start(C lane_top, int top) {
-        const uint64_t mine = order_key(lane_top);
-        int rank = 0;
-        for (int j = 0; j < 32; ++j) {
-            const uint64_t k = __shfl_sync(0xffffffffu, mine, j);
-            rank += k > mine || (k == mine && j < static_cast<int>(threadIdx.x & 31));
-        }
-        const unsigned at_bar = __ballot_sync(0xffffffffu, rank == top - 1);
-        bar = __shfl_sync(0xffffffffu, lane_top, __ffs(at_bar) - 1);
+    __device__ __forceinline__ bool above(Key o) const { return k > o.k; }
+    __device__ __forceinline__ int at() const { return static_cast<int>(~static_cast<uint32_t>(k)); }
+    __device__ __forceinline__ bool none() const { return k == 0; }
+    __device__ __forceinline__ float value() const {
+        const uint32_t o = static_cast<uint32_t>(k >> 32);
+        return o == 0xffffffffu ? NAN : __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
     }
-    // Offers one candidate of every lane (those with `offer`); the whole warp takes part.
-    __device__ __forceinline__ void offer(bool offer, C value, int index, int top) {
-        offer = offer && !(value < bar);
-        if (!__any_sync(0xffffffffu, offer)) return;
-        const int lane = threadIdx.x & 31;
-        const uint64_t mine = offer ? order_key(value) : 0;
-        uint64_t bar_key = __shfl_sync(0xffffffffu, key, top - 1);
-        int bar_at = __shfl_sync(0xffffffffu, at, top - 1);
-        unsigned left = __ballot_sync(0xffffffffu, offer && (mine > bar_key || (mine == bar_key && index < bar_at)));
-        while (left) {
-            const int from = __ffs(left) - 1;
-            left &= left - 1;
-            const uint64_t k = __shfl_sync(0xffffffffu, mine, from);
-            const int i = __shfl_sync(0xffffffffu, index, from);
-            const int rank = __popc(__ballot_sync(0xffffffffu, before(k, i)));
-            const uint64_t up_key = __shfl_up_sync(0xffffffffu, key, 1);
-            const int up_at = __shfl_up_sync(0xffffffffu, at, 1);
-            if (lane > rank) {
-                key = up_key;
-                at = up_at;
-            } else if (lane == rank) {
-                key = k;
-                at = i;
-            }
-        }
-        bar_key = __shfl_sync(0xffffffffu, key, top - 1);
-        if (bar_key != 0) bar = max_nan(bar, value_of(bar_key));
+    __device__ __forceinline__ Key from(int lane) const { return {__shfl_sync(0xffffffffu, k, lane)}; }
+    __device__ __forceinline__ Key across(int mask) const { return {__shfl_xor_sync(0xffffffffu, k, mask)}; }
+};
+template <> struct Key<double> {
+    uint64_t k;
+    uint32_t i;
+    __device__ __forceinline__ static Key make(double v, int at) {
+        const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v + 0.0));
+        return {v != v ? ~0ull : b >> 63 ? ~b : b | (1ull << 63), ~static_cast<uint32_t>(at)};
     }
-    // Merges another list of the same form (lane j offers its (j + 1)-th).
-    __device__ __forceinline__ void merge(uint64_t other_key, int other_at, int top) {
-        const int lane = threadIdx.x & 31;
-        for (int j = 0; j < top; ++j) {
-            const uint64_t k = __shfl_sync(0xffffffffu, other_key, j);
-            const int i = __shfl_sync(0xffffffffu, other_at, j);
-            const int rank = __popc(__ballot_sync(0xffffffffu, before(k, i)));
-            if (rank >= top) return;        // the other's list falls from here on
-            const uint64_t up_key = __shfl_up_sync(0xffffffffu, key, 1);
-            const int up_at = __shfl_up_sync(0xffffffffu, at, 1);
-            if (lane > rank) {
-                key = up_key;
-                at = up_at;
-            } else if (lane == rank) {
-                key = k;
-                at = i;
-            }
-        }
+    __device__ __forceinline__ bool above(Key o) const { return k > o.k || (k == o.k && i > o.i); }
+    __device__ __forceinline__ int at() const { return static_cast<int>(~i); }
+    __device__ __forceinline__ bool none() const { return k == 0; }
+    __device__ __forceinline__ double value() const {
+        return k == ~0ull ? NAN : __longlong_as_double(static_cast<long long>(k >> 63 ? k & 0x7fffffffffffffffull : ~k));
     }
-    static __device__ __forceinline__ C value_of(uint64_t k) {
-        if (k == ~0ull) return NAN;
-        if constexpr (sizeof(C) == 4) {
-            const uint32_t b = static_cast<uint32_t>(k);
-            return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
-        } else {
-            return __longlong_as_double(static_cast<long long>(k >> 63 ? k & 0x7fffffffffffffffull : ~k));
-        }
+    __device__ __forceinline__ Key from(int lane) const { return {__shfl_sync(0xffffffffu, k, lane), __shfl_sync(0xffffffffu, i, lane)}; }
+    __device__ __forceinline__ Key across(int mask) const {
+        return {__shfl_xor_sync(0xffffffffu, k, mask), __shfl_xor_sync(0xffffffffu, i, mask)};
     }
 };
 
-template <int NP, typename C>
+// A warp's best logits so far, lane j holding the (j + 1)-th.  Logits that reach `bar` (no more than the
+// top-th best so far) wait in shared memory until 32 have come, which are then sorted and merged in a
+// bitonic network: 21 exchanges for 32 candidates, where inserting one by one took about ten shuffles each
+// (one row of 128256 words, 20 alternatives: 40 us).
+template <typename C>
+struct Best {
+    Key<C> mine;
+    Key<C>* waiting;         // 64 places of this warp
+    int count;
+    C bar;
+    __device__ __forceinline__ void clear(Key<C>* place) {
+        mine = Key<C>{};
+        waiting = place;
+        count = 0;
+        bar = -INFINITY;
+    }
+    static __device__ __forceinline__ void exchange(Key<C>& k, int mask, bool keep_larger) {
+        const Key<C> o = k.across(mask);
+        if (o.above(k) == keep_larger) k = o;
+    }
+    // Both lists fall from lane 0: the larger of k_j and other_(31 - j) are the best 32 of both, in bitonic order.
+    __device__ __forceinline__ void merge(Key<C> other) {
+        const int lane = threadIdx.x & 31;
+        other = other.across(31);
+        if (other.above(mine)) mine = other;
+#pragma unroll
+        for (int mask = 16; mask > 0; mask >>= 1) exchange(mine, mask, (lane & mask) == 0);
+    }
+    // The first bar from each lane's largest logit: the top-th of them is no more than the top-th logit.
+    __device__ __forceinline__ void start(C lane_top, int top) {
+        Key<C> k = Key<C>::make(lane_top, threadIdx.x & 31);
+        sort(k);
+        bar = k.from(top - 1).value();
+    }
+    static __device__ __forceinline__ void sort(Key<C>& k) {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int size = 2; size <= 32; size <<= 1) {
+#pragma unroll
+            for (int mask = size >> 1; mask > 0; mask >>= 1) exchange(k, mask, ((lane & size) == 0) == ((lane & mask) == 0));
+        }
+    }
+    __device__ __forceinline__ void flush(int top) {
+        const int lane = threadIdx.x & 31;
+        Key<C> k = lane < count ? waiting[lane] : Key<C>{};
+        const Key<C> rest = lane + 32 < count ? waiting[lane + 32] : Key<C>{};
+        __syncwarp();
+        waiting[lane] = rest;
+        count = max(count - 32, 0);
+        __syncwarp();
+        sort(k);
+        merge(k);
+        const Key<C> last = mine.from(top - 1);
+        if (!last.none()) bar = max_nan(bar, last.value());
+    }
+    // One candidate of every lane with `offer`; the whole warp takes part.
+    __device__ __forceinline__ void add(bool offer, C value, int index, int top) {
+        const unsigned who = __ballot_sync(0xffffffffu, offer);
+        if (offer) waiting[count + __popc(who & ((1u << (threadIdx.x & 31)) - 1u))] = Key<C>::make(value, index);
+        count += __popc(who);
+        __syncwarp();
+        if (count >= 32) flush(top);
+    }
+};
+
+template <int NP, typename C, bool TOP>
 struct FwdShared {
     RowSum<NP, C> part[16];
     RowSum<NP, C> block;
-    uint64_t key[16][32];
-    int at[16][32];
+    Key<C> best[TOP ? 16 : 1][64];     // a warp's waiting candidates, then its list
 };
 
 // Groups of a thread that are in flight while as many are worked on: enough bytes to cover the latency of
@@ -355,14 +366,19 @@ struct FwdShared {
 template <int NP>
 constexpr int lp_depth() { return NP == 1 ? 2 : 1; }
 
+// Most threads of a forward block.
+template <int NP>
+constexpr int lp_threads() { return NP > 3 ? 256 : 512; }
+
 // One pass over the logits: the blocks of a cluster (gridDim.x of them, one or more) share a row, each
 // thread keeps the running sums of its groups of 16 bytes per plane, and the parts are joined in the warp,
 // in the block and through distributed shared memory in the cluster's first block.
-template <typename T, int NP>
-__global__ void __launch_bounds__(NP > 6 ? 256 : 512) token_log_probs_fwd_kernel(const __grid_constant__ LogProbParams p) {
+template <typename T, int NP, bool TOP>
+__global__ void __launch_bounds__(lp_threads<NP>(), NP == 4 && !TOP && sizeof(typename Compute<T>::type) == 4 ? 3 : 1)
+token_log_probs_fwd_kernel(const __grid_constant__ LogProbParams p) {
     using C = typename Compute<T>::type;
     constexpr int VEC = lp_vec<T>(), DEPTH = lp_depth<NP>();
-    __shared__ FwdShared<NP, C> sh;
+    __shared__ FwdShared<NP, C, TOP> sh;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int64_t row = blockIdx.y + static_cast<int64_t>(blockIdx.z) * gridDim.y;
     if (row >= p.rows) return;               // the whole cluster
@@ -400,7 +416,7 @@ __global__ void __launch_bounds__(NP > 6 ? 256 : 512) token_log_probs_fwd_kernel
     LogSum<NP, C> sum;
     sum.clear();
     Best<C> best;
-    best.clear();
+    if constexpr (TOP) best.clear(sh.best[warp]);
     for (int base = begin + warp * 32; base < end; base += DEPTH * stride) {
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) now[d] = next[d];
@@ -434,7 +450,7 @@ __global__ void __launch_bounds__(NP > 6 ? 256 : 512) token_log_probs_fwd_kernel
                     sum.add(now[d].v[0].get(i), scale, u);
                 }
             }
-            if (p.top) {
+            if constexpr (TOP) {
                 if (d == 0 && base == begin + warp * 32) best.start(top, p.top);
                 if (__any_sync(0xffffffffu, live && !(top < best.bar))) {
                     unsigned open = 0;
@@ -449,7 +465,7 @@ __global__ void __launch_bounds__(NP > 6 ? 256 : 512) token_log_probs_fwd_kernel
                     while (__any_sync(0xffffffffu, open != 0)) {
                         const int index = g * VEC - groups.skew + __ffs(open) - 1;
                         const C value = open ? to_c<C>(static_cast<const T*>(p.x[0])[row_at + index]) : C(0);
-                        best.offer(open != 0, value, index, p.top);
+                        best.add(open != 0, value, index, p.top);
                         open &= open - 1;
                     }
                 }
@@ -468,38 +484,42 @@ __global__ void __launch_bounds__(NP > 6 ? 256 : 512) token_log_probs_fwd_kernel
     }
     all.join_warp();
     if (lane == 0) sh.part[warp] = all;
-    if (p.top) {
-        sh.key[warp][lane] = best.key;
-        sh.at[warp][lane] = best.at;
+    if constexpr (TOP) {
+        if (best.count) best.flush(p.top);
+        sh.best[warp][lane] = best.mine;
     }
     __syncthreads();
+    if constexpr (TOP)
+        for (int step = 1; step < warps; step *= 2) {        // warps in pairs
+            if (warp % (2 * step) == 0 && warp + step < warps) {
+                best.merge(sh.best[warp + step][lane]);
+                sh.best[warp][lane] = best.mine;
+            }
+            __syncthreads();
+        }
     if (warp == 0) {
         if (lane < warps) all = sh.part[lane];
         else all.clear();
         all.join_warp();
-        if (p.top)
-            for (int w = 1; w < warps; ++w) best.merge(sh.key[w][lane], sh.at[w][lane], p.top);
     }
     if (gridDim.x > 1) {
         namespace cg = cooperative_groups;
         cg::cluster_group cluster = cg::this_cluster();
-        if (warp == 0) {
-            if (lane == 0) sh.block = all;
-            if (p.top) {
-                sh.key[0][lane] = best.key;
-                sh.at[0][lane] = best.at;
-            }
-        }
+        if (threadIdx.x == 0) sh.block = all;
         cluster.sync();
         if (first_block && warp == 0) {
             if (lane < static_cast<int>(gridDim.x)) all = *cluster.map_shared_rank(&sh.block, lane);
             else all.clear();
             all.join_warp();
-            if (p.top)
-                for (unsigned o = 1; o < gridDim.x; ++o) {
-                    const FwdShared<NP, C>* other = cluster.map_shared_rank(&sh, o);
-                    best.merge(other->key[0][lane], other->at[0][lane], p.top);
-                }
+            if constexpr (TOP) {
+                Key<C> other[LP_MAX_SHARE];
+#pragma unroll
+                for (int o = 1; o < LP_MAX_SHARE; ++o)
+                    if (o < static_cast<int>(gridDim.x)) other[o] = cluster.map_shared_rank(&sh, o)->best[0][lane];
+#pragma unroll
+                for (int o = 1; o < LP_MAX_SHARE; ++o)
+                    if (o < static_cast<int>(gridDim.x)) best.merge(other[o]);
+            }
         }
         cluster.sync();                      // the others' shared memory stays until it has been read
     }
@@ -515,11 +535,11 @@ __global__ void __launch_bounds__(NP > 6 ? 256 : 512) token_log_probs_fwd_kernel
     } else {
         s_log<NP, C>(all.S, L);
     }
-    if (lane < p.top) {
+    if (TOP && lane < p.top) {
         C z[NP], v[NP];
-        load_logit<NP, T, C>(p, row, best.at, z);
+        load_logit<NP, T, C>(p, row, best.mine.at(), z);
         log_prob<NP, C>(z, m, L, v);
-        p.top_tokens[row * p.top + lane] = best.at;
+        p.top_tokens[row * p.top + lane] = best.mine.at();
 #pragma unroll
         for (int k = 0; k < NP; ++k)
             if (k < p.np) static_cast<C*>(p.top_logp[k])[row * p.top + lane] = v[k];
@@ -725,8 +745,8 @@ static cudaError_t launch_log_probs(const LogProbParams& p, bool backward, cudaS
     }
     // a row is shared by more blocks while the blocks do not fill the GPU and each keeps a group a thread
     int share = 1;
-    while (share < 8 && p.rows * share < num_sms() && groups / (2 * share) >= 256) share *= 2;
-    const int threads = share > 1 && groups / share >= 1024 && NP <= 6 ? 512 : groups >= 512 ? 256 : 128;
+    while (share < LP_MAX_SHARE && p.rows * share < num_sms() && groups / (2 * share) >= 256) share *= 2;
+    const int threads = share > 1 && groups / share >= 1024 ? lp_threads<NP>() : groups >= 512 ? 256 : 128;
     cudaLaunchConfig_t config{};
     config.gridDim = row_grid(p.rows, share);
     config.blockDim = dim3(threads);
@@ -737,7 +757,8 @@ static cudaError_t launch_log_probs(const LogProbParams& p, bool backward, cudaS
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     config.attrs = &attr;
     config.numAttrs = share > 1 ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&config, token_log_probs_fwd_kernel<T, NP>, p);
+    const cudaError_t e = p.top ? cudaLaunchKernelEx(&config, token_log_probs_fwd_kernel<T, NP, true>, p)
+                                : cudaLaunchKernelEx(&config, token_log_probs_fwd_kernel<T, NP, false>, p);
     note_launch();
     return e;
 }
