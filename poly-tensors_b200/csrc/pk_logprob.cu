@@ -317,11 +317,19 @@ struct Best {
 #pragma unroll
         for (int mask = 16; mask > 0; mask >>= 1) exchange(mine, mask, (lane & mask) == 0);
     }
-    // The first bar from each lane's largest logit: the top-th of them is no more than the top-th logit.
-    __device__ __forceinline__ void start(C lane_top, int top) {
-        Key<C> k = Key<C>::make(lane_top, threadIdx.x & 31);
+    // A first bar from the largest logit of every thread of the block: with j = ceil(top / warps), the
+    // ceil(top / j)-th largest of the warps' j-th largest has at least `top` logits at or above it.  Few
+    // logits pass it (8192 x 32000 bfloat16, 5 alternatives: 428 us with a bar from the warp's own lanes).
+    __device__ __forceinline__ void start(C lane_top, int top, Key<C>* of_warps) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+        const int j = (top + warps - 1) / warps;
+        Key<C> k = Key<C>::make(lane_top, threadIdx.x);
         sort(k);
-        bar = k.from(top - 1).value();
+        if (lane == j - 1) of_warps[warp] = k;
+        __syncthreads();
+        k = lane < warps ? of_warps[lane] : Key<C>{};
+        sort(k);
+        bar = k.from((top + j - 1) / j - 1).value();
     }
     static __device__ __forceinline__ void sort(Key<C>& k) {
         const int lane = threadIdx.x & 31;
@@ -358,13 +366,14 @@ template <int NP, typename C, bool TOP>
 struct FwdShared {
     RowSum<NP, C> part[16];
     RowSum<NP, C> block;
+    Key<C> first[TOP ? 16 : 1];        // a value of each warp for the first bar
     Key<C> best[TOP ? 16 : 1][64];     // a warp's waiting candidates, then its list
 };
 
 // Groups of a thread that are in flight while as many are worked on: enough bytes to cover the latency of
 // memory at low degrees, what the registers allow at high ones.
-template <int NP>
-constexpr int lp_depth() { return NP == 1 ? 2 : 1; }
+template <typename T, int NP, bool TOP>
+constexpr int lp_depth() { return NP == 1 || (NP == 2 && sizeof(T) == 4 && !TOP) ? 2 : 1; }
 
 // Most threads of a forward block.
 template <int NP>
@@ -374,17 +383,17 @@ constexpr int lp_threads() { return NP > 3 ? 256 : 512; }
 // thread keeps the running sums of its groups of 16 bytes per plane, and the parts are joined in the warp,
 // in the block and through distributed shared memory in the cluster's first block.
 template <typename T, int NP, bool TOP>
-__global__ void __launch_bounds__(lp_threads<NP>(), NP == 4 && !TOP && sizeof(typename Compute<T>::type) == 4 ? 3 : 1)
+__global__ void __launch_bounds__(lp_threads<NP>(), sizeof(T) == 8 ? 1 : NP == 4 ? 3 : NP <= 3 && TOP ? 2 : 1)
 token_log_probs_fwd_kernel(const __grid_constant__ LogProbParams p) {
     using C = typename Compute<T>::type;
-    constexpr int VEC = lp_vec<T>(), DEPTH = lp_depth<NP>();
+    constexpr int VEC = lp_vec<T>(), DEPTH = lp_depth<T, NP, TOP>();
     __shared__ FwdShared<NP, C, TOP> sh;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int64_t row = blockIdx.y + static_cast<int64_t>(blockIdx.z) * gridDim.y;
     if (row >= p.rows) return;               // the whole cluster
     const int64_t row_at = row * p.x_rs;
     const bool aligned = p.aligned != 0;
-    RowGroups groups;
+    RowGroups groups{};
     groups.set<T>(static_cast<const T*>(p.x[0]) + row_at, p.cols, aligned);
     // this block's groups, and every thread of a warp the same number of steps
     const int per_block = (groups.count + gridDim.x - 1) / gridDim.x;
@@ -416,7 +425,19 @@ token_log_probs_fwd_kernel(const __grid_constant__ LogProbParams p) {
     LogSum<NP, C> sum;
     sum.clear();
     Best<C> best;
-    if constexpr (TOP) best.clear(sh.best[warp]);
+    if constexpr (TOP) {
+        best.clear(sh.best[warp]);
+        C top = -INFINITY;
+        if (begin + static_cast<int>(threadIdx.x) < end) {
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) {
+                C a, b;
+                next[0].v[0].get(i).get(a, b);
+                top = max_nan(top, max_nan(a, b));
+            }
+        }
+        best.start(top, p.top, sh.first);
+    }
     for (int base = begin + warp * 32; base < end; base += DEPTH * stride) {
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) now[d] = next[d];
@@ -451,7 +472,6 @@ token_log_probs_fwd_kernel(const __grid_constant__ LogProbParams p) {
                 }
             }
             if constexpr (TOP) {
-                if (d == 0 && base == begin + warp * 32) best.start(top, p.top);
                 if (__any_sync(0xffffffffu, live && !(top < best.bar))) {
                     unsigned open = 0;
 #pragma unroll
@@ -596,7 +616,7 @@ __global__ void __launch_bounds__(256) token_log_probs_bwd_kernel(const __grid_c
     RowGrad<NP, C> r;
     r.m = stats[0];
     const bool dead = token == p.ignore_index || r.m == -INFINITY;      // no gradient at all
-    RowGroups groups;
+    RowGroups groups{};
     const T* row0 = static_cast<const T*>(p.x[0]) + x_at;
     bool aligned = p.aligned != 0;
     if (aligned && reinterpret_cast<uintptr_t>(row0) % 16 != reinterpret_cast<uintptr_t>(static_cast<const T*>(p.dx[0]) + dx_at) % 16)
@@ -746,7 +766,10 @@ static cudaError_t launch_log_probs(const LogProbParams& p, bool backward, cudaS
     // a row is shared by more blocks while the blocks do not fill the GPU and each keeps a group a thread
     int share = 1;
     while (share < LP_MAX_SHARE && p.rows * share < num_sms() && groups / (2 * share) >= 256) share *= 2;
-    const int threads = share > 1 && groups / share >= 1024 ? lp_threads<NP>() : groups >= 512 ? 256 : 128;
+    int threads = share > 1 && groups / share >= 1024 ? lp_threads<NP>() : groups >= 512 ? 256 : 128;
+    // many short rows: about four groups a thread, so that a row's join is not most of its work
+    if (p.rows >= 8 * num_sms())
+        while (threads > 32 && groups < 4 * threads) threads /= 2;
     cudaLaunchConfig_t config{};
     config.gridDim = row_grid(p.rows, share);
     config.blockDim = dim3(threads);
