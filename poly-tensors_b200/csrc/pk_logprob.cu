@@ -290,19 +290,20 @@ template <> struct Key<double> {
 };
 
 // A warp's best logits so far, lane j holding the (j + 1)-th.  Logits that reach `bar` (no more than the
-// top-th best so far) wait in shared memory until 32 have come, which are then sorted and merged in a
-// bitonic network: 21 exchanges for 32 candidates, where inserting one by one took about ten shuffles each
-// (one row of 128256 words, 20 alternatives: 40 us).
+// top-th best) wait in shared memory until 32 have come, which are then sorted and merged in a bitonic
+// network: 21 exchanges for 32 candidates.
 template <typename C>
 struct Best {
-    Key<C> mine;
+    Key<C> mine, last;       // last: the list's top-th (nothing while it is not full)
     Key<C>* waiting;         // 64 places of this warp
     int count;
+    bool sorted;             // `mine` holds something
     C bar;
     __device__ __forceinline__ void clear(Key<C>* place) {
-        mine = Key<C>{};
+        mine = last = Key<C>{};
         waiting = place;
         count = 0;
+        sorted = false;
         bar = -INFINITY;
     }
     static __device__ __forceinline__ void exchange(Key<C>& k, int mask, bool keep_larger) {
@@ -317,19 +318,25 @@ struct Best {
 #pragma unroll
         for (int mask = 16; mask > 0; mask >>= 1) exchange(mine, mask, (lane & mask) == 0);
     }
-    // A first bar from the largest logit of every thread of the block: with j = ceil(top / warps), the
-    // ceil(top / j)-th largest of the warps' j-th largest has at least `top` logits at or above it.  Few
-    // logits pass it (8192 x 32000 bfloat16, 5 alternatives: 428 us with a bar from the warp's own lanes).
+    // The bar from the largest logit of every thread of the block: with j = ceil(top / warps), the
+    // ceil(top / j)-th largest of the warps' j-th largest has at least `top` logits at or above it.
     __device__ __forceinline__ void start(C lane_top, int top, Key<C>* of_warps) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-        const int j = (top + warps - 1) / warps;
+        const int j = (top + warps - 1) / warps, want = (top + j - 1) / j - 1;
         Key<C> k = Key<C>::make(lane_top, threadIdx.x);
-        sort(k);
+        if (j == 1) {
+#pragma unroll
+            for (int mask = 16; mask > 0; mask >>= 1) exchange(k, mask, true);
+        } else {
+            sort(k);
+        }
         if (lane == j - 1) of_warps[warp] = k;
         __syncthreads();
         k = lane < warps ? of_warps[lane] : Key<C>{};
-        sort(k);
-        bar = k.from((top + j - 1) / j - 1).value();
+        int rank = lane < warps ? 0 : -1;
+        if (rank == 0)
+            for (int w = 0; w < warps; ++w) rank += of_warps[w].above(k) ? 1 : 0;
+        bar = k.from(__ffs(__ballot_sync(0xffffffffu, rank == want)) - 1).value();
     }
     static __device__ __forceinline__ void sort(Key<C>& k) {
         const int lane = threadIdx.x & 31;
@@ -349,13 +356,16 @@ struct Best {
         __syncwarp();
         sort(k);
         merge(k);
-        const Key<C> last = mine.from(top - 1);
+        sorted = true;
+        last = mine.from(top - 1);
         if (!last.none()) bar = max_nan(bar, last.value());
     }
     // One candidate of every lane with `offer`; the whole warp takes part.
     __device__ __forceinline__ void add(bool offer, C value, int index, int top) {
+        const Key<C> k = Key<C>::make(value, index);
+        offer = offer && k.above(last);
         const unsigned who = __ballot_sync(0xffffffffu, offer);
-        if (offer) waiting[count + __popc(who & ((1u << (threadIdx.x & 31)) - 1u))] = Key<C>::make(value, index);
+        if (offer) waiting[count + __popc(who & ((1u << (threadIdx.x & 31)) - 1u))] = k;
         count += __popc(who);
         __syncwarp();
         if (count >= 32) flush(top);
@@ -367,7 +377,9 @@ struct FwdShared {
     RowSum<NP, C> part[16];
     RowSum<NP, C> block;
     Key<C> first[TOP ? 16 : 1];        // a value of each warp for the first bar
-    Key<C> best[TOP ? 16 : 1][64];     // a warp's waiting candidates, then its list
+    Key<C> best[TOP ? 16 : 1][64];     // a warp's waiting candidates
+    Key<C> list[TOP ? 16 : 1][32];     // its sorted list, where it has one
+    int waiting[TOP ? 16 : 1], sorted[TOP ? 16 : 1];
 };
 
 // Groups of a thread that are in flight while as many are worked on: enough bytes to cover the latency of
@@ -424,20 +436,8 @@ token_log_probs_fwd_kernel(const __grid_constant__ LogProbParams p) {
     const C scale = C(p.scale);
     LogSum<NP, C> sum;
     sum.clear();
-    Best<C> best;
-    if constexpr (TOP) {
-        best.clear(sh.best[warp]);
-        C top = -INFINITY;
-        if (begin + static_cast<int>(threadIdx.x) < end) {
-#pragma unroll
-            for (int i = 0; i < VEC / 2; ++i) {
-                C a, b;
-                next[0].v[0].get(i).get(a, b);
-                top = max_nan(top, max_nan(a, b));
-            }
-        }
-        best.start(top, p.top, sh.first);
-    }
+    C largest = -INFINITY, second = -INFINITY;      // of the thread's groups (NaN above all), and
+    int where = begin + threadIdx.x;                // the group of the first
     for (int base = begin + warp * 32; base < end; base += DEPTH * stride) {
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) now[d] = next[d];
@@ -472,23 +472,10 @@ token_log_probs_fwd_kernel(const __grid_constant__ LogProbParams p) {
                 }
             }
             if constexpr (TOP) {
-                if (__any_sync(0xffffffffu, live && !(top < best.bar))) {
-                    unsigned open = 0;
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) {
-                        C a, b;
-                        now[d].v[0].get(i / 2).get(a, b);
-                        const int index = g * VEC - groups.skew + i;
-                        open |= (live && index >= 0 && index < p.cols && !((i % 2 ? b : a) < best.bar) ? 1u : 0u) << i;
-                    }
-                    // rare: the values are read again, so that this stays one short loop
-                    while (__any_sync(0xffffffffu, open != 0)) {
-                        const int index = g * VEC - groups.skew + __ffs(open) - 1;
-                        const C value = open ? to_c<C>(static_cast<const T*>(p.x[0])[row_at + index]) : C(0);
-                        best.add(open != 0, value, index, p.top);
-                        open &= open - 1;
-                    }
-                }
+                const bool up = top > largest || top != top;
+                second = max_nan(second, up ? largest : top);
+                where = up ? g : where;
+                largest = max_nan(largest, top);
             }
         }
     }
@@ -504,19 +491,74 @@ token_log_probs_fwd_kernel(const __grid_constant__ LogProbParams p) {
     }
     all.join_warp();
     if (lane == 0) sh.part[warp] = all;
+    Best<C> best;
     if constexpr (TOP) {
-        if (best.count) best.flush(p.top);
-        sh.best[warp][lane] = best.mine;
+        // Only threads whose largest logit reaches the bar can hold an alternative (a few of the block).  They
+        // read that logit's group again, and the rest of theirs only where the second largest reaches it too.
+        best.clear(sh.best[warp]);
+        best.start(largest, p.top, sh.first);
+        const bool look = !(largest < best.bar), everywhere = look && !(second < best.bar);
+        if (__any_sync(0xffffffffu, look)) {
+            const auto examine = [&](bool here, int g) {
+                Group<1, T> again;
+                unsigned open = 0;
+                if (here) {
+                    again.load(p, row_at, groups, g);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        C a, b;
+                        again.v[0].get(i / 2).get(a, b);
+                        const int index = g * VEC - groups.skew + i;
+                        open |= (index >= 0 && index < p.cols && !((i % 2 ? b : a) < best.bar) ? 1u : 0u) << i;
+                    }
+                }
+                while (__any_sync(0xffffffffu, open != 0)) {
+                    const int i = __ffs(open) - 1;
+                    C value = C(0);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) {
+                        C a, b;
+                        again.v[0].get(j / 2).get(a, b);
+                        if (j == i) value = j % 2 ? b : a;
+                    }
+                    best.add(open != 0, value, g * VEC - groups.skew + i, p.top);
+                    open &= open - 1;
+                }
+            };
+            const bool mine = begin + static_cast<int>(threadIdx.x) < end;
+            examine(look && mine, where);
+            if (__any_sync(0xffffffffu, everywhere))
+                for (int base = begin + warp * 32; base < end; base += stride) {
+                    const int g = base + lane;
+                    examine(everywhere && g < end && g != where, g);
+                }
+        }
+        if (best.sorted) sh.list[warp][lane] = best.mine;
+        if (lane == 0) {
+            sh.waiting[warp] = best.count;
+            sh.sorted[warp] = best.sorted;
+        }
     }
     __syncthreads();
-    if constexpr (TOP)
-        for (int step = 1; step < warps; step *= 2) {        // warps in pairs
-            if (warp % (2 * step) == 0 && warp + step < warps) {
-                best.merge(sh.best[warp + step][lane]);
-                sh.best[warp][lane] = best.mine;
+    if constexpr (TOP) {
+        // the first warp takes what all have: the waiting candidates 32 at a time, and the others' lists
+        if (warp == 0) {
+            int count = 0;
+            for (int w = 0; w < warps; ++w) count += sh.waiting[w];
+            for (int base = 0; base < count; base += 32) {
+                int at = base + lane;
+                Key<C> k{};
+                for (int w = 0; w < warps; ++w) {
+                    if (at >= 0 && at < sh.waiting[w]) k = sh.best[w][at];
+                    at -= sh.waiting[w];
+                }
+                Best<C>::sort(k);
+                best.merge(k);
             }
-            __syncthreads();
+            for (int w = 1; w < warps; ++w)
+                if (sh.sorted[w]) best.merge(sh.list[w][lane]);
         }
+    }
     if (warp == 0) {
         if (lane < warps) all = sh.part[lane];
         else all.clear();
@@ -526,6 +568,7 @@ token_log_probs_fwd_kernel(const __grid_constant__ LogProbParams p) {
         namespace cg = cooperative_groups;
         cg::cluster_group cluster = cg::this_cluster();
         if (threadIdx.x == 0) sh.block = all;
+        if (TOP && warp == 0) sh.list[0][lane] = best.mine;
         cluster.sync();
         if (first_block && warp == 0) {
             if (lane < static_cast<int>(gridDim.x)) all = *cluster.map_shared_rank(&sh.block, lane);
@@ -535,7 +578,7 @@ token_log_probs_fwd_kernel(const __grid_constant__ LogProbParams p) {
                 Key<C> other[LP_MAX_SHARE];
 #pragma unroll
                 for (int o = 1; o < LP_MAX_SHARE; ++o)
-                    if (o < static_cast<int>(gridDim.x)) other[o] = cluster.map_shared_rank(&sh, o)->best[0][lane];
+                    if (o < static_cast<int>(gridDim.x)) other[o] = cluster.map_shared_rank(&sh, o)->list[0][lane];
 #pragma unroll
                 for (int o = 1; o < LP_MAX_SHARE; ++o)
                     if (o < static_cast<int>(gridDim.x)) best.merge(other[o]);
