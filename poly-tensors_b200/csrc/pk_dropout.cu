@@ -8,7 +8,7 @@
 // is formed in float (double for float64 planes) and rounded once, when it is stored.
 #include <algorithm>
 
-#include "pk_rows.cuh"
+#include "pk_vec.cuh"
 
 namespace pk {
 
@@ -40,9 +40,9 @@ __device__ __forceinline__ uint4 philox4x32_10(uint64_t counter, uint64_t offset
     return make_uint4(c0, c1, c2, c3);
 }
 
-// One thread per counter (four consecutive elements) and step, all planes.
+// Planes whose bases lie on no 16-byte boundary: one thread per counter (four consecutive elements).
 template <typename T>
-__global__ void __launch_bounds__(256) dropout_kernel(const DropoutParams p) {
+__global__ void __launch_bounds__(256) dropout_scalar_kernel(const DropoutParams p) {
     using C = typename Compute<T>::type;
     const C scale = C(p.scale);
     const int64_t groups = (p.n + 3) / 4;
@@ -63,11 +63,100 @@ __global__ void __launch_bounds__(256) dropout_kernel(const DropoutParams p) {
     }
 }
 
+// Elements of a thread: whole counters, and vectors of 16 bytes.
+template <typename T>
+constexpr int dropout_unit() { return sizeof(T) == 2 ? 8 : 4; }
+
+// Vector form, bound by memory traffic: a thread asks for its 16-byte vectors of every plane of x and the
+// residual, forms their counters' words (ten rounds, about 90 instructions for four elements of every plane)
+// while they are on the way, and writes.  Measured on B200, device time: see the launch below.
+template <typename T, int NP>
+__global__ void __launch_bounds__(256) dropout_vec_kernel(const __grid_constant__ DropoutParams p) {
+    using C = typename Compute<T>::type;
+    constexpr int UNIT = dropout_unit<T>(), VEC = 16 / sizeof(T), PARTS = UNIT / VEC, WORDS = UNIT / 4;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+    const int64_t first = i * UNIT;
+    if (first >= p.n) return;
+    const bool whole = first + UNIT <= p.n;
+    Raw<T, VEC> x[NP][PARTS], r[NP][PARTS];
+    if (whole) {
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+#pragma unroll
+            for (int v = 0; v < PARTS; ++v) {
+                if (k < p.nx) x[k][v] = *reinterpret_cast<const Raw<T, VEC>*>(static_cast<const T*>(p.x[k]) + first + v * VEC);
+                if (k < p.nr) r[k][v] = *reinterpret_cast<const Raw<T, VEC>*>(static_cast<const T*>(p.residual[k]) + first + v * VEC);
+            }
+        }
+    }
+    uint32_t word[UNIT];
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) {
+        const uint4 q = philox4x32_10(static_cast<uint64_t>(i) * WORDS + w, p.offset, p.seed);
+        word[4 * w] = q.x;
+        word[4 * w + 1] = q.y;
+        word[4 * w + 2] = q.z;
+        word[4 * w + 3] = q.w;
+    }
+    const C scale = C(p.scale);
+    if (!whole) {                     // the last elements
+        for (int k = 0; k < p.np; ++k) {
+#pragma unroll
+            for (int u = 0; u < UNIT; ++u) {
+                if (first + u >= p.n) break;
+                C v = C(0);
+                if (k < p.nx && word[u] >= p.threshold) v = to_c<C>(static_cast<const T*>(p.x[k])[first + u]) * scale;
+                if (k < p.nr) v += to_c<C>(static_cast<const T*>(p.residual[k])[first + u]);
+                static_cast<T*>(p.y[k])[first + u] = from_c<T>(v);
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+        if (NP > 6 && k >= p.np) continue;
+#pragma unroll
+        for (int v = 0; v < PARTS; ++v) {
+            Raw<T, VEC> out;
+#pragma unroll
+            for (int j = 0; j < VEC / 2; ++j) {
+                C a = C(0), b = C(0), c = C(0), d = C(0);
+                if (k < p.nx) x[k][v].get(j).get(a, b);
+                if (k < p.nr) r[k][v].get(j).get(c, d);
+                a = word[v * VEC + 2 * j] >= p.threshold ? a : C(0);
+                b = word[v * VEC + 2 * j + 1] >= p.threshold ? b : C(0);
+                out.set(j, fma2(Two<C>(a, b), Two<C>(scale), Two<C>(c, d)));
+            }
+            *reinterpret_cast<Raw<T, VEC>*>(static_cast<T*>(p.y[k]) + first + v * VEC) = out;
+        }
+    }
+}
+
+template <typename T, int NP>
+static void launch_dropout_vec(const DropoutParams& p, cudaStream_t s) {
+    const int64_t blocks = ceil_div(ceil_div(p.n, dropout_unit<T>()), 256);
+    PK_LAUNCHED(dropout_vec_kernel<T, NP><<<static_cast<unsigned>(blocks), 256, 0, s>>>(p));
+}
+
 template <typename T>
 static void launch_dropout(const DropoutParams& p, cudaStream_t s) {
-    const int64_t groups = ceil_div(p.n, 4);
-    const int grid = static_cast<int>(std::min<int64_t>(ceil_div(groups, 256), static_cast<int64_t>(num_sms()) * 32));
-    PK_LAUNCHED(dropout_kernel<T><<<grid, 256, 0, s>>>(p));
+    const bool aligned = planes_aligned(p.x, p.nx, 16) && planes_aligned(p.residual, p.nr, 16) && planes_aligned(p.y, p.np, 16);
+    if (!aligned || p.n > (1ll << 40)) {
+        const int64_t groups = ceil_div(p.n, 4);
+        const int grid = static_cast<int>(std::min<int64_t>(ceil_div(groups, 256), static_cast<int64_t>(num_sms()) * 32));
+        PK_LAUNCHED(dropout_scalar_kernel<T><<<grid, 256, 0, s>>>(p));
+        return;
+    }
+    switch (p.np) {
+        case 1: launch_dropout_vec<T, 1>(p, s); break;
+        case 2: launch_dropout_vec<T, 2>(p, s); break;
+        case 3: launch_dropout_vec<T, 3>(p, s); break;
+        case 4: launch_dropout_vec<T, 4>(p, s); break;
+        case 5: launch_dropout_vec<T, 5>(p, s); break;
+        case 6: launch_dropout_vec<T, 6>(p, s); break;
+        case 7: case 8: case 9: launch_dropout_vec<T, 9>(p, s); break;
+        default: launch_dropout_vec<T, 16>(p, s); break;
+    }
 }
 
 }  // namespace pk
