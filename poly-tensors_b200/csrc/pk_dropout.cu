@@ -19,12 +19,15 @@ struct DropoutParams {
     int np, nx, nr;          // planes of y, x and the residual (missing ones are zero)
     int64_t n;               // elements of a plane
     uint64_t seed, offset;
-    uint64_t threshold;      // 0 .. 2^32
+    uint32_t threshold;      // (a threshold of 2^32 drops everything: nx is 0 then)
     double scale;
 };
 
-__device__ __forceinline__ uint4 philox4x32_10(uint64_t counter, uint64_t offset, uint64_t seed) {
-    uint32_t c0 = static_cast<uint32_t>(counter), c1 = static_cast<uint32_t>(counter >> 32);
+// Philox4x32-10 of the counter (i, offset), i of 64 or (HIGH false) of 32 bits.  The second product of the first
+// round, and with 32-bit i the first of the second, are the same for all threads of a launch.
+template <bool HIGH>
+__device__ __forceinline__ uint4 philox4x32_10(uint64_t i, uint64_t offset, uint64_t seed) {
+    uint32_t c0 = static_cast<uint32_t>(i), c1 = HIGH ? static_cast<uint32_t>(i >> 32) : 0u;
     uint32_t c2 = static_cast<uint32_t>(offset), c3 = static_cast<uint32_t>(offset >> 32);
     uint32_t k0 = static_cast<uint32_t>(seed), k1 = static_cast<uint32_t>(seed >> 32);
 #pragma unroll
@@ -40,7 +43,7 @@ __device__ __forceinline__ uint4 philox4x32_10(uint64_t counter, uint64_t offset
     return make_uint4(c0, c1, c2, c3);
 }
 
-// Planes whose bases lie on no 16-byte boundary: one thread per counter (four consecutive elements).
+// Planes whose bases lie on no 16-byte boundary, and more than 2^34 elements: one thread per counter (four consecutive elements).
 template <typename T>
 __global__ void __launch_bounds__(256) dropout_scalar_kernel(const DropoutParams p) {
     using C = typename Compute<T>::type;
@@ -48,7 +51,7 @@ __global__ void __launch_bounds__(256) dropout_scalar_kernel(const DropoutParams
     const int64_t groups = (p.n + 3) / 4;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < groups;
          i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        const uint4 words = philox4x32_10(static_cast<uint64_t>(i), p.offset, p.seed);
+        const uint4 words = philox4x32_10<true>(static_cast<uint64_t>(i), p.offset, p.seed);
         const uint32_t word[4] = {words.x, words.y, words.z, words.w};
         for (int k = 0; k < p.np; ++k) {
             for (int u = 0; u < 4; ++u) {
@@ -92,7 +95,7 @@ __global__ void __launch_bounds__(256) dropout_vec_kernel(const __grid_constant_
     uint32_t word[UNIT];
 #pragma unroll
     for (int w = 0; w < WORDS; ++w) {
-        const uint4 q = philox4x32_10(static_cast<uint64_t>(i) * WORDS + w, p.offset, p.seed);
+        const uint4 q = philox4x32_10<false>(static_cast<uint64_t>(i) * WORDS + w, p.offset, p.seed);
         word[4 * w] = q.x;
         word[4 * w + 1] = q.y;
         word[4 * w + 2] = q.z;
@@ -141,7 +144,7 @@ static void launch_dropout_vec(const DropoutParams& p, cudaStream_t s) {
 template <typename T>
 static void launch_dropout(const DropoutParams& p, cudaStream_t s) {
     const bool aligned = planes_aligned(p.x, p.nx, 16) && planes_aligned(p.residual, p.nr, 16) && planes_aligned(p.y, p.np, 16);
-    if (!aligned || p.n > (1ll << 40)) {
+    if (!aligned || p.n > (1ll << 34)) {
         const int64_t groups = ceil_div(p.n, 4);
         const int grid = static_cast<int>(std::min<int64_t>(ceil_div(groups, 256), static_cast<int64_t>(num_sms()) * 32));
         PK_LAUNCHED(dropout_scalar_kernel<T><<<grid, 256, 0, s>>>(p));
@@ -175,12 +178,12 @@ extern "C" int pk_dropout(int dtype, int degree, int64_t n, const void* const* x
         return fail(PK_ERR_ARG, "pk_dropout: bad plane count");
     if (!x || !y || (residual_planes && !residual)) return fail(PK_ERR_ARG, "pk_dropout: null plane array");
     if (n == 0) return PK_OK;
-    p.nx = x_planes;
+    p.nx = threshold >> 32 ? 0 : x_planes;
     p.nr = residual_planes;
     p.n = n;
     p.seed = seed;
     p.offset = offset;
-    p.threshold = threshold;
+    p.threshold = static_cast<uint32_t>(threshold);
     p.scale = scale;
     for (int k = 0; k < p.np; ++k) {
         if (k < p.nx) p.x[k] = x[k];
