@@ -337,6 +337,7 @@ def attention_decomposed(query, key, value, attn_mask=None, dropout_p=0.0, is_ca
 _RMS_NORM = frozenset((F.rms_norm, torch.rms_norm))
 _CROSS_ENTROPY = frozenset((F.cross_entropy,))
 _ATTENTION = frozenset((F.scaled_dot_product_attention,))
+INTERCEPTED = _RMS_NORM | _CROSS_ENTROPY | _ATTENTION   # what maybe_fused looks at
 _CE_ARGS = ("input", "target", "weight", "size_average", "ignore_index", "reduce", "reduction", "label_smoothing")
 _SDPA_ARGS = ("query", "key", "value", "attn_mask", "dropout_p", "is_causal", "scale", "enable_gqa")
 

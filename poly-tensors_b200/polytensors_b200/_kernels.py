@@ -17,7 +17,9 @@ _DTYPE_CODE = {torch.float32: _lib.PK_F32, torch.float64: _lib.PK_F64,
 
 
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    """The handle of the current stream on a device."""
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def _require_cuda(tensors, what):
@@ -627,9 +629,21 @@ def cross_entropy_bwd(z_planes, target, ignore_index, softcap, stats, g_planes):
 
 def _unit_inner(planes):
     """Planes sharing one stride pattern whose last stride is 1."""
-    if _same_strides(planes) and (planes[0].stride(-1) == 1 or planes[0].shape[-1] == 1):
-        return planes
+    strides = planes[0].stride()
+    if strides[-1] == 1 or planes[0].shape[-1] == 1:
+        for p in planes[1:]:
+            if p.stride() != strides:
+                break
+        else:
+            return planes
     return [p.contiguous() for p in planes]
+
+
+def _as(planes, dtype, shape):
+    """Gradient planes of a type and shape (autograd may hand over expanded or wider ones)."""
+    if planes[0].dtype == dtype and planes[0].shape == shape:
+        return planes
+    return [p.to(dtype).expand(shape) for p in planes]
 
 
 def _qk_args(q, k, qw, kw, plan):
@@ -638,57 +652,58 @@ def _qk_args(q, k, qw, kw, plan):
     B, T, H, D = q[0].shape
     q, k = _unit_inner(q), _unit_inner(k)
     qw, kw = [w.contiguous() for w in qw], [w.contiguous() for w in kw]
-    arrays = [_lib.pointer_array(x) for x in (q, k, qw, kw)]
-    head = [dtype_code(q[0].dtype), len(q) - 1, B, T, H, k[0].shape[2], D, 2 * cos.shape[1], int(interleaved)]
-    tail = [arrays[0][0], *q[0].stride()[:3], arrays[1][0], *k[0].stride()[:3], arrays[2][0], len(qw),
-            arrays[3][0], len(kw), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
-            positions.data_ptr() if positions is not None else None,
+    pq, pk, pqw, pkw = (_lib.pointer_array(x)[0] for x in (q, k, qw, kw))
+    args = [dtype_code(q[0].dtype), len(q) - 1, B, T, H, k[0].shape[2], D, 2 * cos.shape[1], int(interleaved),
+            pq, *q[0].stride()[:3], pk, *k[0].stride()[:3], pqw, len(qw), pkw, len(kw), cos.data_ptr(),
+            sin.data_ptr(), cos.shape[0], None if positions is None else positions.data_ptr(),
             T if positions is not None and positions.dim() == 2 else 0, eps]
-    return head, tail, (q, k, qw, kw, arrays)
+    return args, (q, k, qw, kw)
 
 
 def qk_norm_rope_fwd(q, k, qw, kw, plan):
     """Normalised and rotated heads (B, H, T, D) of q (B, T, H, D) and of k, all planes
     (pk_qk_norm_rope_fwd).  qw / kw: weight planes, [] for none; plan: (cos, sin, positions, eps,
     interleaved) with tables in the compute type and contiguous int64 positions or None."""
-    head, tail, alive = _qk_args(q, k, qw, kw, plan)
-    B, T, _, D = q[0].shape
-    outs = [[torch.empty(B, x[0].shape[2], T, D, dtype=x[0].dtype, device=x[0].device) for _ in x] for x in (q, k)]
-    pq, k1 = _lib.pointer_array(outs[0])
-    pk, k2 = _lib.pointer_array(outs[1])
-    status = _lib.load().pk_qk_norm_rope_fwd(*head, *tail, pq, pk, _stream(q[0].device))
+    args, alive = _qk_args(q, k, qw, kw, plan)
+    B, T, H, D = q[0].shape
+    new, shape = q[0].new_empty, (B, H, T, D)
+    q_out = [new(shape) for _ in q]
+    shape = (B, k[0].shape[2], T, D)
+    k_out = [new(shape) for _ in k]
+    status = _lib.load().pk_qk_norm_rope_fwd(*args, _lib.pointer_array(q_out)[0], _lib.pointer_array(k_out)[0],
+                                             _stream(q[0].device))
     _lib.check(status, "pk_qk_norm_rope_fwd")
-    return outs
+    return q_out, k_out
 
 
 def qk_norm_rope_bwd(q, k, qw, kw, gq, gk, plan, want_dqw, want_dkw):
     """(dq, dk, dqw, dkw) from the outputs' gradients (None: that output was not used, and its side is
     skipped).  Weight gradients have as many planes as their weight."""
     lib = _lib.load()
-    head, tail, alive = _qk_args(q, k, qw, kw, plan)
-    dtype, degree, B, T = head[:4]
-    grads, strides, outs, sums = [], [], [], []
+    args, alive = _qk_args(q, k, qw, kw, plan)
+    dtype, degree, B, T = args[:4]
+    new, dt = q[0].new_empty, q[0].dtype
+    grads, outs, sums, counts, passed = [], [], [], [], []
     for i, (x, g, w, want) in enumerate(((q, gq, qw, want_dqw), (k, gk, kw, want_dkw))):
         if g is None:
-            head[4 + i] = 0
-            grads.append(None)
-            strides.append((0, 0, 0))
-            outs.append(None)
-            sums.append(None)
-            continue
-        D = x[0].shape[-1]
-        g = _unit_inner([p.to(x[0].dtype).expand(B, x[0].shape[2], T, D) for p in g])
+            args[4 + i] = 0
+            out = dw = None
+            passed += [None, 0, 0, 0]
+        else:
+            H, D = x[0].shape[2:]
+            g = _unit_inner(_as(g, dt, (B, H, T, D)))
+            shape = x[0].shape
+            out = [new(shape) for _ in x]
+            dw = [new(D) for _ in w] if want and w else None
+            passed += [_lib.pointer_array(g)[0], *g[0].stride()[:3]]
         grads.append(g)
-        strides.append(g[0].stride()[:3])
-        outs.append([torch.empty(x[0].shape, dtype=x[0].dtype, device=x[0].device) for _ in x])
-        sums.append([torch.empty(D, dtype=x[0].dtype, device=x[0].device) for _ in w] if want and w else None)
-    counts = [len(s) if s else 0 for s in sums]
-    need = lib.pk_qk_norm_rope_bwd_workspace_size(dtype, degree, B, T, *head[4:7], *counts)
+        outs.append(out)
+        sums.append(dw)
+        counts.append(len(dw) if dw else 0)
+    need = lib.pk_qk_norm_rope_bwd_workspace_size(dtype, degree, B, T, *args[4:7], *counts) if any(counts) else 0
     ws = torch.empty(need, dtype=torch.uint8, device=q[0].device) if need else None
-    arrays = [_lib.pointer_array(x) if x else (None, None) for x in (*grads, *outs, *sums)]
-    status = lib.pk_qk_norm_rope_bwd(*head, *tail, arrays[0][0], *strides[0], arrays[1][0], *strides[1],
-                                     *(a[0] for a in arrays[2:]), ws.data_ptr() if ws is not None else None, need,
-                                     _stream(q[0].device))
+    passed += [_lib.pointer_array(x)[0] if x else None for x in (*outs, *sums)]
+    status = lib.pk_qk_norm_rope_bwd(*args, *passed, ws.data_ptr() if need else None, need, _stream(q[0].device))
     _lib.check(status, "pk_qk_norm_rope_bwd")
     return (*outs, *sums)
 
@@ -697,13 +712,11 @@ def dropout(x, residual, planes, p, seed, offset):
     """``planes`` output planes residual + keep * x / (1 - p) (pk_dropout); x and residual may have fewer
     (missing ones are zero)."""
     x, residual = [t.contiguous() for t in x], [t.contiguous() for t in residual]
-    out = [torch.empty(x[0].shape, dtype=x[0].dtype, device=x[0].device) for _ in range(planes)]
-    px, k1 = _lib.pointer_array(x)
-    pr, k2 = _lib.pointer_array(residual)
-    po, k3 = _lib.pointer_array(out)
-    threshold = int(p * 2.0 ** 32)
-    status = _lib.load().pk_dropout(dtype_code(x[0].dtype), planes - 1, x[0].numel(), px, len(x), pr, len(residual),
-                                    threshold, 1.0 / (1.0 - p) if p < 1.0 else 0.0, seed, offset, po,
+    new, shape = x[0].new_empty, x[0].shape
+    out = [new(shape) for _ in range(planes)]
+    status = _lib.load().pk_dropout(dtype_code(x[0].dtype), planes - 1, x[0].numel(), _lib.pointer_array(x)[0], len(x),
+                                    _lib.pointer_array(residual)[0], len(residual), int(p * 2.0 ** 32),
+                                    1.0 / (1.0 - p) if p < 1.0 else 0.0, seed, offset, _lib.pointer_array(out)[0],
                                     _stream(x[0].device))
     _lib.check(status, "pk_dropout")
     return out
@@ -713,16 +726,20 @@ def token_log_probs_fwd(z, tokens, ignore_index, scale, top):
     """(log_probs, entropy, top_log_probs, top_tokens, stats) of (R, V) logits planes and (R,) int64
     tokens (pk_token_log_probs_fwd); the alternatives are None without ``top``."""
     z, tokens = _unit_inner(z), tokens.contiguous()
-    (R, V), dev, cdt = z[0].shape, z[0].device, compute_dtype(z[0].dtype)
-    logp, entropy = ([torch.empty(R, dtype=cdt, device=dev) for _ in z] for _ in range(2))
-    top_logp = [torch.empty(R, top, dtype=cdt, device=dev) for _ in z] if top else None
-    top_tokens = torch.empty(R, top, dtype=torch.int64, device=dev) if top else None
-    stats = torch.empty(R, len(z) + 1, dtype=cdt, device=dev)
-    arrays = [_lib.pointer_array(t) if t else (None, None) for t in (z, logp, entropy, top_logp)]
+    first = z[0]
+    (R, V), n, dev, cdt = first.shape, len(z), first.device, compute_dtype(first.dtype)
+    stats = torch.empty(R, n + 1, dtype=cdt, device=dev)
+    new = stats.new_empty
+    logp, entropy = [new(R) for _ in z], [new(R) for _ in z]
+    top_logp = top_tokens = None
+    if top:
+        top_logp = [new((R, top)) for _ in z]
+        top_tokens = tokens.new_empty((R, top))
+    pointers = _lib.pointer_array
     status = _lib.load().pk_token_log_probs_fwd(
-        dtype_code(z[0].dtype), len(z) - 1, R, V, arrays[0][0], z[0].stride(0), tokens.data_ptr(), ignore_index,
-        scale, top, arrays[1][0], arrays[2][0], arrays[3][0], top_tokens.data_ptr() if top else None,
-        stats.data_ptr(), _stream(dev))
+        dtype_code(first.dtype), n - 1, R, V, pointers(z)[0], first.stride(0), tokens.data_ptr(), ignore_index, scale,
+        top, pointers(logp)[0], pointers(entropy)[0], pointers(top_logp)[0] if top else None,
+        top_tokens.data_ptr() if top else None, stats.data_ptr(), _stream(dev))
     _lib.check(status, "pk_token_log_probs_fwd")
     return logp, entropy, top_logp, top_tokens, stats
 
@@ -730,13 +747,15 @@ def token_log_probs_fwd(z, tokens, ignore_index, scale, top):
 def token_log_probs_bwd(z, tokens, ignore_index, scale, top, stats, entropy, top_tokens, grads):
     """dlogits planes (R, V) from the gradients of (log_probs, entropy, top_log_probs), None for none."""
     z, tokens = _unit_inner(z), tokens.contiguous()
-    (R, V), dev = z[0].shape, z[0].device
+    first = z[0]
+    (R, V), n = first.shape, len(z)
     flat = [None if g is None else [p.to(stats.dtype).contiguous() for p in g] for g in grads]
-    dz = [torch.empty(R, V, dtype=z[0].dtype, device=dev) for _ in z]
-    arrays = [_lib.pointer_array(t) if t else (None, None) for t in (z, entropy, *flat, dz)]
+    new = first.new_empty
+    dz = [new((R, V)) for _ in z]
+    pointers = _lib.pointer_array
     status = _lib.load().pk_token_log_probs_bwd(
-        dtype_code(z[0].dtype), len(z) - 1, R, V, arrays[0][0], z[0].stride(0), tokens.data_ptr(), ignore_index,
-        scale, top, stats.data_ptr(), arrays[1][0], top_tokens.data_ptr() if top else None, arrays[2][0],
-        arrays[3][0], arrays[4][0], arrays[5][0], V, _stream(dev))
+        dtype_code(first.dtype), n - 1, R, V, pointers(z)[0], first.stride(0), tokens.data_ptr(), ignore_index, scale,
+        top, stats.data_ptr(), pointers(entropy)[0], top_tokens.data_ptr() if top else None,
+        *[pointers(g)[0] if g else None for g in flat], pointers(dz)[0], V, _stream(first.device))
     _lib.check(status, "pk_token_log_probs_bwd")
     return dz

@@ -182,11 +182,21 @@ def launch_count(reset=False):
     return load().pk_launch_count(1 if reset else 0)
 
 
+# Array types by length: ctypes passes an array where a pointer to its element type is declared.
+_POINTERS = [ctypes.c_void_p * n for n in range(2 * PK_MAX_PLANES + 1)]
+_INTEGERS = [ctypes.c_int64 * max(n, 1) for n in range(2 * PK_MAX_PLANES + 1)]
+
+
 def pointer_array(tensors):
-    arr = (ctypes.c_void_p * len(tensors))(*[t.data_ptr() if t is not None else None for t in tensors])
-    return ctypes.cast(arr, _pp), arr
+    """The host array of the planes' addresses, twice (what to pass, and what to keep alive until then)."""
+    n = len(tensors)
+    kind = _POINTERS[n] if n < len(_POINTERS) else ctypes.c_void_p * n
+    arr = kind(*[t.data_ptr() if t is not None else None for t in tensors])
+    return arr, arr
 
 
 def int64_array(values):
-    arr = (ctypes.c_int64 * max(len(values), 1))(*values)
-    return ctypes.cast(arr, _p64), arr
+    n = len(values)
+    kind = _INTEGERS[n] if n < len(_INTEGERS) else ctypes.c_int64 * n
+    arr = kind(*values)
+    return arr, arr

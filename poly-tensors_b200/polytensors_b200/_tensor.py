@@ -14,7 +14,7 @@ import operator
 
 import torch
 
-from . import _state
+from . import _fused, _state, _token_ops
 from ._dispatch import dispatch
 
 # Complex dtype that may carry the directions of a real constant coefficient.
@@ -25,22 +25,46 @@ def _shares_memory(a, b):
     return torch._C._overlaps(a, b)
 
 
+def _memory_apart(planes):
+    """Whether no two planes share memory: by their address ranges when all are contiguous (and have
+    elements), pair by pair otherwise."""
+    starts, size = [], 0
+    for c in planes:
+        if not c.is_contiguous():
+            break
+        starts.append(c.data_ptr())
+        size = max(size, c.nbytes)
+    else:
+        starts.sort()
+        if size and all([b - a >= size for a, b in zip(starts, starts[1:])]):
+            return True
+    return not any(_shares_memory(planes[i], planes[j]) for i in range(1, len(planes)) for j in range(i))
+
+
 def _is_canonical(planes):
     """True when ``planes`` can be used as they are: plain dense tensors on one device with one
     shape, a floating or complex constant coefficient, every higher coefficient of a single
     dtype (the constant's, or its complex counterpart), and no two coefficients sharing memory."""
-    if not planes or any(type(c) is not torch.Tensor or c.layout != torch.strided for c in planes):
+    if not planes:
         return False
-    head, rest = planes[0], planes[1:]
-    if not (head.dtype.is_floating_point or head.dtype.is_complex):
+    head = planes[0]
+    if type(head) is not torch.Tensor or head.layout != torch.strided:
         return False
-    if any(c.shape != head.shape or c.device != head.device for c in rest):
+    kind = head.dtype
+    if not (kind.is_floating_point or kind.is_complex):
         return False
-    if rest:
-        kinds = {c.dtype for c in rest}
-        if len(kinds) != 1 or kinds.pop() not in (head.dtype, _DIRECTION_DTYPE.get(head.dtype)):
+    if len(planes) == 1:
+        return True
+    shape, device = head.shape, head.device
+    for c in planes[1:]:
+        if type(c) is not torch.Tensor or c.layout != torch.strided or c.shape != shape or c.device != device:
             return False
-    return not any(_shares_memory(planes[i], planes[j]) for i in range(1, len(planes)) for j in range(i))
+    direction = planes[1].dtype
+    if direction != kind and direction != _DIRECTION_DTYPE.get(kind):
+        return False
+    if any(c.dtype != direction for c in planes[2:]):
+        return False
+    return _memory_apart(planes)
 
 
 def _degree_argument(degree):
@@ -146,7 +170,11 @@ class PolyTensor(torch.Tensor):
 
     @staticmethod
     def __new__(cls, coeffs, *, degree=None, requires_grad=False):
-        planes = _planes_from(coeffs, degree)
+        return cls._of(_planes_from(coeffs, degree), requires_grad)
+
+    @classmethod
+    def _of(cls, planes, requires_grad=False):
+        """The wrapper around a tuple of planes that meet the constructor's rules as they are."""
         head = planes[0]
         self = torch.Tensor._make_wrapper_subclass(
             cls, head.shape, strides=head.stride(), storage_offset=head.storage_offset(), dtype=head.dtype,
@@ -272,10 +300,8 @@ class PolyTensor(torch.Tensor):
         """Queries (B, T, H, D) and keys (B, T, K, D) normalised per head and rotated by position in
         one pass, returned head-major for attention (see ``_token_ops.qk_norm_rope``).  Accepts
         ordinary tensors and PolyTensors (no counterpart in the reference)."""
-        from ._token_ops import qk_norm_rope
-
-        return qk_norm_rope(query, key, query_weight, key_weight, cos, sin, positions=positions, eps=eps,
-                            interleaved=interleaved, check_indices=check_indices)
+        return _token_ops.qk_norm_rope(query, key, query_weight, key_weight, cos, sin, positions=positions, eps=eps,
+                                       interleaved=interleaved, check_indices=check_indices)
 
     @staticmethod
     def dropout(input, p, seed, offset=0, residual=None):
@@ -283,19 +309,15 @@ class PolyTensor(torch.Tensor):
         element's index, the same for every coefficient, formed again in backward (see
         ``_token_ops.dropout``).  Accepts ordinary tensors and PolyTensors (no counterpart in the
         reference)."""
-        from ._token_ops import dropout
-
-        return dropout(input, p, seed, offset=offset, residual=residual)
+        return _token_ops.dropout(input, p, seed, offset=offset, residual=residual)
 
     @staticmethod
     def token_log_probs(logits, tokens, top=0, temperature=1.0, ignore_index=-100, check_indices=True):
         """Log probabilities of given tokens, entropy and best alternatives of (..., V) logits in one
         pass, differentiable (see ``_token_ops.token_log_probs``).  Accepts ordinary tensors and
         PolyTensors (no counterpart in the reference)."""
-        from ._token_ops import token_log_probs
-
-        return token_log_probs(logits, tokens, top=top, temperature=temperature, ignore_index=ignore_index,
-                               check_indices=check_indices)
+        return _token_ops.token_log_probs(logits, tokens, top=top, temperature=temperature,
+                                          ignore_index=ignore_index, check_indices=check_indices)
 
     def backward(self, gradient=None, retain_graph=None, create_graph=False, inputs=None):
         """Reverse-mode through the series: the seed is ``gradient`` as a PolyTensor of this degree
@@ -325,11 +347,10 @@ class PolyTensor(torch.Tensor):
     @classmethod
     def __torch_function__(cls, func, types, args=(), kwargs=None):
         kwargs = {} if kwargs is None else kwargs
-        from ._fused import maybe_fused
-
-        result = maybe_fused(func, args, kwargs)
-        if result is not NotImplemented:
-            return result
+        if func in _fused.INTERCEPTED:
+            result = _fused.maybe_fused(func, args, kwargs)
+            if result is not NotImplemented:
+                return result
         with torch._C.DisableTorchFunctionSubclass():
             return func(*args, **kwargs)
 

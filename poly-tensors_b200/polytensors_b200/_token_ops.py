@@ -8,6 +8,7 @@ degree 0; next to PolyTensors it is a constant (zero higher planes).  Unsupporte
 ``NotImplementedError``, wrong shapes and values ``ValueError``, indices out of range ``IndexError``.
 """
 
+import functools
 import operator
 from typing import NamedTuple
 
@@ -27,32 +28,69 @@ class TokenLogProbs(NamedTuple):
     top_tokens: torch.Tensor
 
 
-def _degree(what, *operands):
-    """The common degree of the PolyTensors among the operands (None when all are ordinary tensors)."""
-    P = _state.poly_cls()
+def _public(fn):
+    """A public call: runs with PolyTensor's interception off, so that reading an operand's attributes costs
+    no Python call (the operators handle the planes themselves)."""
+
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        with torch._C.DisableTorchFunctionSubclass():
+            return fn(*args, **kwargs)
+
+    return call
+
+
+def _operands(what, *operands):
+    """The planes of each operand ([] for None; an ordinary tensor is its own one plane), the common degree
+    of the PolyTensors among them (None without any), and the PolyTensor class.  All planes are real
+    floating-point tensors of one type on one device."""
+    cls = _state.poly_cls()
     if _state.coefficient_autograd.get():
         raise NotImplementedError(f"{what}: not available in PolyTensor.coefficient_autograd()")
-    degrees = {x.degree for x in operands if isinstance(x, P)}
-    if len(degrees) > 1:
-        raise ValueError("PolyTensor operands must have the same degree")
-    degree = degrees.pop() if degrees else None
+    planes, degree, dtype, device = [], None, None, None
+    for x in operands:
+        if x is None:
+            planes.append([])
+            continue
+        if isinstance(x, cls):
+            if degree is not None and x.degree != degree:
+                raise ValueError("PolyTensor operands must have the same degree")
+            degree, own = x.degree, list(x.coeffs)
+        elif isinstance(x, torch.Tensor):
+            own = [x]
+        else:
+            raise TypeError(f"{what}: expected tensors, got {type(x).__name__}")
+        for p in own:
+            if dtype is None:
+                dtype, device = p.dtype, p.device
+                K.dtype_code(dtype)
+            elif p.dtype != dtype:
+                raise NotImplementedError(f"{what}: operands of differing types ({dtype} and {p.dtype})")
+            elif p.device != device:
+                raise ValueError(f"{what}: operands on differing devices ({device} and {p.device})")
+        planes.append(own)
     if degree is not None and degree >= _lib.PK_MAX_PLANES:
         raise NotImplementedError(f"{what}: degree {degree} exceeds {_lib.PK_MAX_PLANES - 1}")
-    return degree
+    return planes, degree, cls
 
 
-def _coeffs(x):
-    """A series' planes; an ordinary tensor is its own one plane."""
-    return list(x.coeffs) if isinstance(x, _state.poly_cls()) else [x]
+def _require_cuda(what, tensor):
+    if not tensor.is_cuda:
+        K._require_cuda([tensor], what)
 
 
 def _full(planes, degree):
     """The planes with the zero ones of a constant filled in."""
-    return planes + [torch.zeros_like(planes[0]) for _ in range((degree or 0) + 1 - len(planes))]
+    missing = (degree or 0) + 1 - len(planes)
+    return planes + [torch.zeros_like(planes[0]) for _ in range(missing)] if missing else planes
 
 
 def _wrap(planes, degree, cls):
-    return planes[0] if degree is None else cls(tuple(planes))
+    """A kernel's output planes as the caller's kind of variable."""
+    if degree is None:
+        return planes[0]
+    of = getattr(cls, "_of", cls)       # another PolyTensor class: through its constructor
+    return of(tuple(planes))
 
 
 def _grad_planes(g, degree, cls):
@@ -62,22 +100,8 @@ def _grad_planes(g, degree, cls):
     return _full(list(g.coeffs) if isinstance(g, cls) else [g], degree)
 
 
-def _check_planes(what, planes, dtype=None, device=None):
-    """Every plane a real floating CUDA tensor of one type (``dtype``) on one device."""
-    dtype, device = dtype or planes[0].dtype, device or planes[0].device
-    for p in planes:
-        if not isinstance(p, torch.Tensor):
-            raise TypeError(f"{what}: expected tensors, got {type(p).__name__}")
-        K.dtype_code(p.dtype)
-        if p.dtype != dtype:
-            raise NotImplementedError(f"{what}: operands of differing types ({dtype} and {p.dtype})")
-        if p.device != device:
-            raise ValueError(f"{what}: operands on differing devices ({device} and {p.device})")
-    K._require_cuda(planes, what)
-
-
-def _check_index_tensor(what, idx, device):
-    if isinstance(idx, _state.poly_cls()) or not isinstance(idx, torch.Tensor):
+def _check_index_tensor(what, idx, device, cls):
+    if isinstance(idx, cls) or not isinstance(idx, torch.Tensor):
         raise TypeError(f"{what} must be an ordinary integer tensor")
     if idx.is_floating_point() or idx.is_complex() or idx.dtype == torch.bool:
         raise TypeError(f"{what} must be integers, got {idx.dtype}")
@@ -105,15 +129,11 @@ class _QKNormRope(torch.autograd.Function):
     """(q', k') from (q, k): one launch forward, one and the weight sums backward."""
 
     @staticmethod
-    def forward(ctx, query, key, q_weight, k_weight, degree, plan):
-        cls = _state.poly_cls()
-        Q, Kp = _full(_coeffs(query), degree), _full(_coeffs(key), degree)
-        QW = _coeffs(q_weight) if q_weight is not None else []
-        KW = _coeffs(k_weight) if k_weight is not None else []
-        q_out, k_out = K.qk_norm_rope_fwd(Q, Kp, QW, KW, plan)
+    def forward(ctx, query, key, q_weight, k_weight, planes, degree, cls, plan):
+        q_out, k_out = K.qk_norm_rope_fwd(*planes, plan)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(*Q, *Kp, *QW, *KW)
-        ctx.counts = (len(Q), len(Kp), len(QW), len(KW))
+        ctx.save_for_backward(*planes[0], *planes[1], *planes[2], *planes[3])
+        ctx.counts = [len(p) for p in planes]
         ctx.plan, ctx.degree, ctx.cls = plan, degree, cls
         ctx.poly = [isinstance(x, cls) for x in (query, key, q_weight, k_weight)]
         return _wrap(q_out, degree, cls), _wrap(k_out, degree, cls)
@@ -128,15 +148,16 @@ class _QKNormRope(torch.autograd.Function):
         Q, Kp, QW, KW = groups
         GQ, GK = (_grad_planes(g, ctx.degree, ctx.cls) for g in (gq, gk))
         if GQ is None and GK is None:
-            return (None,) * 6
+            return (None,) * 8
         need = ctx.needs_input_grad
         dq, dk, dqw, dkw = K.qk_norm_rope_bwd(Q, Kp, QW, KW, GQ, GK, ctx.plan, need[2], need[3])
         grads = []
         for planes, poly, wanted in zip((dq, dk, dqw, dkw), ctx.poly, need):
-            grads.append(None if planes is None or not wanted else ctx.cls(tuple(planes)) if poly else planes[0])
-        return (*grads, None, None)
+            grads.append(None if planes is None or not wanted else _wrap(planes, ctx.degree if poly else None, ctx.cls))
+        return (*grads, None, None, None, None)
 
 
+@_public
 def qk_norm_rope(query, key, query_weight, key_weight, cos, sin, positions=None, eps=1e-6, interleaved=False,
                  check_indices=True):
     """Normalise queries and keys per head and rotate them by position, in one pass.
@@ -155,26 +176,25 @@ def qk_norm_rope(query, key, query_weight, key_weight, cos, sin, positions=None,
     become NaN.
     """
     what = "qk_norm_rope"
-    degree = _degree(what, query, key, query_weight, key_weight)
     for name, x in (("query", query), ("key", key)):
         if not isinstance(x, torch.Tensor) or x.dim() != 4:
             raise ValueError(f"{what}: {name} must be (batch, tokens, heads, features)")
-    B, T, _, D = query.shape
-    if key.shape[:2] != (B, T) or key.shape[3] != D:
+    planes, degree, cls = _operands(what, query, key, query_weight, key_weight)
+    first = planes[0][0]
+    device, (B, T, _, D) = first.device, first.shape
+    KB, KT, _, KD = planes[1][0].shape
+    if (KB, KT, KD) != (B, T, D):
         raise ValueError(f"{what}: query {tuple(query.shape)} and key {tuple(key.shape)} differ beyond their heads")
     if not 1 <= D <= 1024:
         raise NotImplementedError(f"{what}: head dimension {D} (1 to 1024)")
-    planes = _coeffs(query) + _coeffs(key)
-    for name, w in (("query_weight", query_weight), ("key_weight", key_weight)):
-        if w is None:
-            continue
-        if not isinstance(w, torch.Tensor) or tuple(w.shape) != (D,):
+    for name, w in (("query_weight", planes[2]), ("key_weight", planes[3])):
+        if w and tuple(w[0].shape) != (D,):
             raise ValueError(f"{what}: {name} must have shape ({D},)")
-        planes += _coeffs(w)
-    _check_planes(what, planes)
-    dtype, device = planes[0].dtype, planes[0].device
+    _require_cuda(what, first)
+    table = K.compute_dtype(first.dtype)
+    tables = []
     for name, t in (("cos", cos), ("sin", sin)):
-        if isinstance(t, _state.poly_cls()) or not isinstance(t, torch.Tensor) or not t.is_floating_point():
+        if isinstance(t, cls) or not isinstance(t, torch.Tensor) or not t.is_floating_point():
             raise TypeError(f"{what}: {name} must be an ordinary floating-point tensor")
         if t.dim() != 2 or t.shape != cos.shape or 2 * t.shape[1] > D:
             raise ValueError(f"{what}: cos and sin must be (positions, at most {D // 2})")
@@ -182,25 +202,22 @@ def qk_norm_rope(query, key, query_weight, key_weight, cos, sin, positions=None,
             raise ValueError(f"{what}: {name} must be on {device}, got {t.device}")
         if t.requires_grad:
             raise NotImplementedError(f"{what}: the angle tables take no gradient")
+        tables.append(t.to(table).contiguous())
     if positions is None:
         if T > cos.shape[0]:
             raise IndexError(f"{what}: {T} tokens need {T} table rows, got {cos.shape[0]}")
     else:
-        _check_index_tensor(f"{what}: positions", positions, device)
+        _check_index_tensor(f"{what}: positions", positions, device, cls)
         if tuple(positions.shape) not in ((T,), (B, T)):
             raise ValueError(f"{what}: positions must be ({T},) or ({B}, {T}), got {tuple(positions.shape)}")
         if check_indices:
             K._check_indices(positions, cos.shape[0], f"{what} position")
         positions = positions.to(torch.int64).contiguous()
-    table = K.compute_dtype(dtype)
-    plan = (cos.to(table).contiguous(), sin.to(table).contiguous(), positions, float(eps), bool(interleaved))
+    plan = (*tables, positions, float(eps), bool(interleaved))
+    planes = [_full(planes[0], degree), _full(planes[1], degree), planes[2], planes[3]]
     if _wants_grad(query, key, query_weight, key_weight):
-        return _QKNormRope.apply(query, key, query_weight, key_weight, degree, plan)
-    with torch.no_grad():
-        q_out, k_out = K.qk_norm_rope_fwd(_full(_coeffs(query), degree), _full(_coeffs(key), degree),
-                                          _coeffs(query_weight) if query_weight is not None else [],
-                                          _coeffs(key_weight) if key_weight is not None else [], plan)
-    cls = _state.poly_cls()
+        return _QKNormRope.apply(query, key, query_weight, key_weight, planes, degree, cls, plan)
+    q_out, k_out = K.qk_norm_rope_fwd(*planes, plan)
     return _wrap(q_out, degree, cls), _wrap(k_out, degree, cls)
 
 
@@ -211,36 +228,38 @@ class _Dropout(torch.autograd.Function):
     """y = residual + dropout(x); the gradient of x is the same dropout of y's."""
 
     @staticmethod
-    def forward(ctx, x, residual, degree, p, seed, offset):
-        cls = _state.poly_cls()
-        X = _coeffs(x)
-        R = _coeffs(residual) if residual is not None else []
-        y = K.dropout(X, R, (degree or 0) + 1, p, seed, offset)
+    def forward(ctx, x, residual, planes, degree, cls, p, seed, offset):
+        y = K.dropout(*planes, (degree or 0) + 1, p, seed, offset)
         ctx.set_materialize_grads(False)
-        ctx.args, ctx.cls = (degree, p, seed, offset), cls
+        ctx.args = (degree, cls, p, seed, offset)
         ctx.poly = (isinstance(x, cls), isinstance(residual, cls))
         return _wrap(y, degree, cls)
 
     @staticmethod
     def backward(ctx, g):
         if g is None:
-            return (None,) * 6
-        degree, p, seed, offset = ctx.args
-        is_poly = isinstance(g, ctx.cls)
+            return (None,) * 8
+        degree, cls, p, seed, offset = ctx.args
 
-        def as_input(series, poly):
-            return series if poly == isinstance(series, ctx.cls) else series.value if not poly \
-                else ctx.cls.constant(series, degree)
+        def as_input(poly):
+            """The gradient for an input that is a series, or an ordinary tensor (its constant plane)."""
+            if poly == isinstance(g, cls):
+                return g
+            return cls.constant(g, degree) if poly else g.coeffs[0]
 
-        dx = dr = None
+        dx = None
         if ctx.needs_input_grad[0]:
-            gx = as_input(g, ctx.poly[0])
-            dx = _Dropout.apply(gx, None, degree if ctx.poly[0] else None, p, seed, offset)
-        if ctx.needs_input_grad[1]:
-            dr = as_input(g, ctx.poly[1])
-        return dx, dr, None, None, None, None
+            gx, own = as_input(ctx.poly[0]), degree if ctx.poly[0] else None
+            planes = [list(gx.coeffs) if ctx.poly[0] else [gx], []]
+            if torch.is_grad_enabled():
+                dx = _Dropout.apply(gx, None, planes, own, cls, p, seed, offset)
+            else:
+                dx = _wrap(K.dropout(*planes, (own or 0) + 1, p, seed, offset), own, cls)
+        dr = as_input(ctx.poly[1]) if ctx.needs_input_grad[1] else None
+        return dx, dr, None, None, None, None, None, None
 
 
+@_public
 def dropout(input, p, seed, offset=0, residual=None):
     """Dropout with a mask from a counter-based generator, optionally added to ``residual``:
     ``residual + keep * input / (1 - p)``, every plane under the same mask, in one pass.
@@ -251,52 +270,53 @@ def dropout(input, p, seed, offset=0, residual=None):
     ``p`` = 0 keeps everything, 1 drops everything.  ``residual`` has the input's shape and type.
     """
     what = "dropout"
-    degree = _degree(what, input, residual)
     if isinstance(p, torch.Tensor) or not 0.0 <= float(p) <= 1.0:
         raise ValueError(f"{what}: p must be a number in [0, 1], got {p}")
     p, seed, offset = float(p), _u64(seed, f"{what}: seed"), _u64(offset, f"{what}: offset")
-    if not isinstance(input, torch.Tensor):
-        raise TypeError(f"{what}: expected a tensor, got {type(input).__name__}")
-    planes = _coeffs(input)
-    if residual is not None:
-        if not isinstance(residual, torch.Tensor) or residual.shape != input.shape:
-            raise ValueError(f"{what}: the residual must have the input's shape {tuple(input.shape)}")
-        planes = planes + _coeffs(residual)
-    _check_planes(what, planes)
+    if residual is not None and (not isinstance(residual, torch.Tensor) or not isinstance(input, torch.Tensor)
+                                 or residual.shape != input.shape):
+        raise ValueError(f"{what}: the residual must have the input's shape")
+    planes, degree, cls = _operands(what, input, residual)
+    if not planes[0]:
+        raise TypeError(f"{what}: expected a tensor, got None")
+    _require_cuda(what, planes[0][0])
     if _wants_grad(input, residual):
-        return _Dropout.apply(input, residual, degree, p, seed, offset)
-    with torch.no_grad():
-        y = K.dropout(_coeffs(input), _coeffs(residual) if residual is not None else [], (degree or 0) + 1, p, seed,
-                      offset)
-    return _wrap(y, degree, _state.poly_cls())
+        return _Dropout.apply(input, residual, planes, degree, cls, p, seed, offset)
+    y = K.dropout(*planes, (degree or 0) + 1, p, seed, offset)
+    return _wrap(y, degree, cls)
 
 
 # ======================================================================================
 # Token log probabilities
 
+def _shaped(out, lead, top, degree, cls):
+    """The kernel's flat results as the caller sees them."""
+    logp, entropy, top_logp, top_tokens = out[:4]
+    if len(lead) != 1:
+        logp, entropy = ([t.view(lead) for t in planes] for planes in (logp, entropy))
+        if top:
+            top_logp, top_tokens = [t.view(*lead, top) for t in top_logp], top_tokens.view(*lead, top)
+    return (_wrap(logp, degree, cls), _wrap(entropy, degree, cls),
+            _wrap(top_logp, degree, cls) if top else None, top_tokens)
+
+
 class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, tokens, degree, ignore_index, scale, top):
-        cls = _state.poly_cls()
-        Z = [z.reshape(-1, z.shape[-1]) for z in _coeffs(logits)]
-        out = K.token_log_probs_fwd(Z, tokens.reshape(-1), ignore_index, scale, top)
-        logp, entropy, top_logp, top_tokens, stats = out
+    def forward(ctx, logits, planes, tokens, lead, degree, cls, ignore_index, scale, top):
+        out = K.token_log_probs_fwd(planes, tokens, ignore_index, scale, top)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(*Z, *entropy, tokens.reshape(-1), stats, *([top_tokens] if top else []))
-        ctx.args, ctx.degree, ctx.cls, ctx.shape = (ignore_index, scale, top), degree, cls, logits.shape
-        lead = tuple(tokens.shape)
-        shaped = [_wrap([t.view(lead) for t in planes], degree, cls) for planes in (logp, entropy)]
-        if not top:
-            return (*shaped, None, None)
-        top_tokens = top_tokens.view(*lead, top)
-        ctx.mark_non_differentiable(top_tokens)
-        return (*shaped, _wrap([t.view(*lead, top) for t in top_logp], degree, cls), top_tokens)
+        ctx.save_for_backward(*planes, *out[1], tokens, out[4], *([out[3]] if top else []))
+        ctx.args, ctx.degree, ctx.cls, ctx.lead = (ignore_index, scale, top), degree, cls, lead
+        results = _shaped(out, lead, top, degree, cls)
+        if top:
+            ctx.mark_non_differentiable(results[3])
+        return results
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_logp, g_entropy, g_top, _):
         if g_logp is None and g_entropy is None and g_top is None:
-            return (None,) * 6
+            return (None,) * 9
         n = (ctx.degree or 0) + 1
         saved = ctx.saved_tensors
         Z, entropy, tokens, stats = saved[:n], saved[n:2 * n], saved[2 * n], saved[2 * n + 1]
@@ -304,9 +324,12 @@ class _TokenLogProbs(torch.autograd.Function):
         grads = [_grad_planes(g, ctx.degree, ctx.cls) for g in (g_logp, g_entropy, g_top)]
         dz = K.token_log_probs_bwd(list(Z), tokens, ignore_index, scale, top, stats, list(entropy),
                                    saved[-1] if top else None, grads)
-        return (_wrap([t.view(ctx.shape) for t in dz], ctx.degree, ctx.cls),) + (None,) * 5
+        if len(ctx.lead) != 1:
+            dz = [t.view(*ctx.lead, t.shape[-1]) for t in dz]
+        return (_wrap(dz, ctx.degree, ctx.cls),) + (None,) * 8
 
 
+@_public
 def token_log_probs(logits, tokens, top=0, temperature=1.0, ignore_index=-100, check_indices=True):
     """Log probabilities of given tokens, with the distribution's entropy and its best alternatives.
 
@@ -322,16 +345,16 @@ def token_log_probs(logits, tokens, top=0, temperature=1.0, ignore_index=-100, c
     check (and its wait for the GPU): such rows' log probabilities then become NaN.
     """
     what = "token_log_probs"
-    degree = _degree(what, logits)
     if not isinstance(logits, torch.Tensor) or logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"{what}: logits must be (..., V) with V >= 1")
-    planes = _coeffs(logits)
-    _check_planes(what, planes)
-    _check_index_tensor(f"{what}: tokens", tokens, planes[0].device)
-    if tokens.shape != logits.shape[:-1]:
-        raise ValueError(f"{what}: tokens {tuple(tokens.shape)} must match the logits' rows "
-                         f"{tuple(logits.shape[:-1])}")
-    V = logits.shape[-1]
+    (planes,), degree, cls = _operands(what, logits)
+    first = planes[0]
+    _require_cuda(what, first)
+    _check_index_tensor(f"{what}: tokens", tokens, first.device, cls)
+    shape, lead = first.shape, tuple(tokens.shape)
+    if lead != tuple(shape[:-1]):
+        raise ValueError(f"{what}: tokens {lead} must match the logits' rows {tuple(shape[:-1])}")
+    V = shape[-1]
     top = operator.index(top)
     if not 0 <= top <= min(32, V):
         raise ValueError(f"{what}: top must lie in [0, {min(32, V)}], got {top}")
@@ -342,15 +365,10 @@ def token_log_probs(logits, tokens, top=0, temperature=1.0, ignore_index=-100, c
     if check_indices:
         K._check_indices(tokens, V, f"{what} token", ignore=ignore_index)
     tokens = tokens.to(torch.int64)
+    if len(lead) != 1:
+        planes, tokens = [z.reshape(-1, V) for z in planes], tokens.reshape(-1)
     scale = 1.0 / temperature
     if _wants_grad(logits):
-        return TokenLogProbs(*_TokenLogProbs.apply(logits, tokens, degree, ignore_index, scale, top))
-    with torch.no_grad():
-        logp, entropy, top_logp, top_tokens, _ = K.token_log_probs_fwd(
-            [z.reshape(-1, V) for z in planes], tokens.reshape(-1), ignore_index, scale, top)
-    cls, lead = _state.poly_cls(), tuple(tokens.shape)
-    shaped = [_wrap([t.view(lead) for t in x], degree, cls) for x in (logp, entropy)]
-    if not top:
-        return TokenLogProbs(*shaped, None, None)
-    return TokenLogProbs(*shaped, _wrap([t.view(*lead, top) for t in top_logp], degree, cls),
-                         top_tokens.view(*lead, top))
+        return TokenLogProbs(*_TokenLogProbs.apply(logits, planes, tokens, lead, degree, cls, ignore_index, scale, top))
+    out = K.token_log_probs_fwd(planes, tokens, ignore_index, scale, top)
+    return TokenLogProbs(*_shaped(out, lead, top, degree, cls))
