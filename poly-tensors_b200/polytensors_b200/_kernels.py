@@ -7,6 +7,7 @@ eager-PyTorch fallback.
 """
 
 import ctypes
+import math
 
 import torch
 
@@ -639,6 +640,25 @@ def _unit_inner(planes):
     return [p.contiguous() for p in planes]
 
 
+def _dense(planes):
+    """The planes, contiguous."""
+    for p in planes:
+        if not p.is_contiguous():
+            return [p.contiguous() for p in planes]
+    return planes
+
+
+_SMALL = 1 << 20
+
+
+def _outputs(like, count, shape):
+    """``count`` uninitialised tensors like another: small ones (up to 1 MiB) in one allocation, whose host
+    time would otherwise exceed the kernel's, larger ones each in its own, to be freed one by one."""
+    if math.prod(shape) * like.itemsize <= _SMALL:
+        return list(like.new_empty((count, *shape)).unbind(0))
+    return [like.new_empty(shape) for _ in range(count)]
+
+
 def _as(planes, dtype, shape):
     """Gradient planes of a type and shape (autograd may hand over expanded or wider ones)."""
     if planes[0].dtype == dtype and planes[0].shape == shape:
@@ -651,7 +671,7 @@ def _qk_args(q, k, qw, kw, plan):
     cos, sin, positions, eps, interleaved = plan
     B, T, H, D = q[0].shape
     q, k = _unit_inner(q), _unit_inner(k)
-    qw, kw = [w.contiguous() for w in qw], [w.contiguous() for w in kw]
+    qw, kw = _dense(qw), _dense(kw)
     pq, pk, pqw, pkw = (_lib.pointer_array(x)[0] for x in (q, k, qw, kw))
     args = [dtype_code(q[0].dtype), len(q) - 1, B, T, H, k[0].shape[2], D, 2 * cos.shape[1], int(interleaved),
             pq, *q[0].stride()[:3], pk, *k[0].stride()[:3], pqw, len(qw), pkw, len(kw), cos.data_ptr(),
@@ -666,10 +686,8 @@ def qk_norm_rope_fwd(q, k, qw, kw, plan):
     interleaved) with tables in the compute type and contiguous int64 positions or None."""
     args, alive = _qk_args(q, k, qw, kw, plan)
     B, T, H, D = q[0].shape
-    new, shape = q[0].new_empty, (B, H, T, D)
-    q_out = [new(shape) for _ in q]
-    shape = (B, k[0].shape[2], T, D)
-    k_out = [new(shape) for _ in k]
+    q_out = _outputs(q[0], len(q), (B, H, T, D))
+    k_out = _outputs(k[0], len(k), (B, k[0].shape[2], T, D))
     status = _lib.load().pk_qk_norm_rope_fwd(*args, _lib.pointer_array(q_out)[0], _lib.pointer_array(k_out)[0],
                                              _stream(q[0].device))
     _lib.check(status, "pk_qk_norm_rope_fwd")
@@ -682,7 +700,7 @@ def qk_norm_rope_bwd(q, k, qw, kw, gq, gk, plan, want_dqw, want_dkw):
     lib = _lib.load()
     args, alive = _qk_args(q, k, qw, kw, plan)
     dtype, degree, B, T = args[:4]
-    new, dt = q[0].new_empty, q[0].dtype
+    dt = q[0].dtype
     grads, outs, sums, counts, passed = [], [], [], [], []
     for i, (x, g, w, want) in enumerate(((q, gq, qw, want_dqw), (k, gk, kw, want_dkw))):
         if g is None:
@@ -692,9 +710,8 @@ def qk_norm_rope_bwd(q, k, qw, kw, gq, gk, plan, want_dqw, want_dkw):
         else:
             H, D = x[0].shape[2:]
             g = _unit_inner(_as(g, dt, (B, H, T, D)))
-            shape = x[0].shape
-            out = [new(shape) for _ in x]
-            dw = [new(D) for _ in w] if want and w else None
+            out = _outputs(x[0], len(x), x[0].shape)
+            dw = _outputs(x[0], len(w), (D,)) if want and w else None
             passed += [_lib.pointer_array(g)[0], *g[0].stride()[:3]]
         grads.append(g)
         outs.append(out)
@@ -711,9 +728,8 @@ def qk_norm_rope_bwd(q, k, qw, kw, gq, gk, plan, want_dqw, want_dkw):
 def dropout(x, residual, planes, p, seed, offset):
     """``planes`` output planes residual + keep * x / (1 - p) (pk_dropout); x and residual may have fewer
     (missing ones are zero)."""
-    x, residual = [t.contiguous() for t in x], [t.contiguous() for t in residual]
-    new, shape = x[0].new_empty, x[0].shape
-    out = [new(shape) for _ in range(planes)]
+    x, residual = _dense(x), _dense(residual)
+    out = _outputs(x[0], planes, x[0].shape)
     status = _lib.load().pk_dropout(dtype_code(x[0].dtype), planes - 1, x[0].numel(), _lib.pointer_array(x)[0], len(x),
                                     _lib.pointer_array(residual)[0], len(residual), int(p * 2.0 ** 32),
                                     1.0 / (1.0 - p) if p < 1.0 else 0.0, seed, offset, _lib.pointer_array(out)[0],
@@ -729,11 +745,10 @@ def token_log_probs_fwd(z, tokens, ignore_index, scale, top):
     first = z[0]
     (R, V), n, dev, cdt = first.shape, len(z), first.device, compute_dtype(first.dtype)
     stats = torch.empty(R, n + 1, dtype=cdt, device=dev)
-    new = stats.new_empty
-    logp, entropy = [new(R) for _ in z], [new(R) for _ in z]
+    logp, entropy = _outputs(stats, n, (R,)), _outputs(stats, n, (R,))
     top_logp = top_tokens = None
     if top:
-        top_logp = [new((R, top)) for _ in z]
+        top_logp = _outputs(stats, n, (R, top))
         top_tokens = tokens.new_empty((R, top))
     pointers = _lib.pointer_array
     status = _lib.load().pk_token_log_probs_fwd(
@@ -749,9 +764,8 @@ def token_log_probs_bwd(z, tokens, ignore_index, scale, top, stats, entropy, top
     z, tokens = _unit_inner(z), tokens.contiguous()
     first = z[0]
     (R, V), n = first.shape, len(z)
-    flat = [None if g is None else [p.to(stats.dtype).contiguous() for p in g] for g in grads]
-    new = first.new_empty
-    dz = [new((R, V)) for _ in z]
+    flat = [None if g is None else _dense(g if g[0].dtype == stats.dtype else [p.to(stats.dtype) for p in g]) for g in grads]
+    dz = _outputs(first, n, (R, V))
     pointers = _lib.pointer_array
     status = _lib.load().pk_token_log_probs_bwd(
         dtype_code(first.dtype), n - 1, R, V, pointers(z)[0], first.stride(0), tokens.data_ptr(), ignore_index, scale,

@@ -25,19 +25,7 @@ def _shares_memory(a, b):
     return torch._C._overlaps(a, b)
 
 
-def _memory_apart(planes):
-    """Whether no two planes share memory: by their address ranges when all are contiguous (and have
-    elements), pair by pair otherwise."""
-    starts, size = [], 0
-    for c in planes:
-        if not c.is_contiguous():
-            break
-        starts.append(c.data_ptr())
-        size = max(size, c.nbytes)
-    else:
-        starts.sort()
-        if size and all([b - a >= size for a, b in zip(starts, starts[1:])]):
-            return True
+def _pairs_apart(planes):
     return not any(_shares_memory(planes[i], planes[j]) for i in range(1, len(planes)) for j in range(i))
 
 
@@ -55,16 +43,32 @@ def _is_canonical(planes):
         return False
     if len(planes) == 1:
         return True
-    shape, device = head.shape, head.device
+    shape, device, direction = head.shape, head.device, None
+    # contiguous planes are told apart by their address ranges, others pair by pair
+    starts = [head.data_ptr()] if head.is_contiguous() else None
     for c in planes[1:]:
         if type(c) is not torch.Tensor or c.layout != torch.strided or c.shape != shape or c.device != device:
             return False
-    direction = planes[1].dtype
-    if direction != kind and direction != _DIRECTION_DTYPE.get(kind):
-        return False
-    if any(c.dtype != direction for c in planes[2:]):
-        return False
-    return _memory_apart(planes)
+        if direction is None:
+            direction = c.dtype
+            if direction != kind and direction != _DIRECTION_DTYPE.get(kind):
+                return False
+        elif c.dtype != direction:
+            return False
+        if starts is not None:
+            if c.is_contiguous():
+                starts.append(c.data_ptr())
+            else:
+                starts = None
+    if starts is not None:
+        starts.sort()
+        size, last = max(head.nbytes, planes[1].nbytes), None
+        for at in starts:
+            if not size or (last is not None and at - last < size):
+                return _pairs_apart(planes)
+            last = at
+        return True
+    return _pairs_apart(planes)
 
 
 def _degree_argument(degree):

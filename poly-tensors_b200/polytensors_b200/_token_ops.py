@@ -110,7 +110,11 @@ def _check_index_tensor(what, idx, device, cls):
 
 
 def _wants_grad(*operands):
-    return torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in operands)
+    if torch.is_grad_enabled():
+        for x in operands:
+            if x is not None and x.requires_grad:
+                return True
+    return False
 
 
 def _u64(value, what):
@@ -183,12 +187,12 @@ def qk_norm_rope(query, key, query_weight, key_weight, cos, sin, positions=None,
     first = planes[0][0]
     device, (B, T, _, D) = first.device, first.shape
     KB, KT, _, KD = planes[1][0].shape
-    if (KB, KT, KD) != (B, T, D):
+    if KB != B or KT != T or KD != D:
         raise ValueError(f"{what}: query {tuple(query.shape)} and key {tuple(key.shape)} differ beyond their heads")
     if not 1 <= D <= 1024:
         raise NotImplementedError(f"{what}: head dimension {D} (1 to 1024)")
     for name, w in (("query_weight", planes[2]), ("key_weight", planes[3])):
-        if w and tuple(w[0].shape) != (D,):
+        if w and w[0].shape != (D,):
             raise ValueError(f"{what}: {name} must have shape ({D},)")
     _require_cuda(what, first)
     table = K.compute_dtype(first.dtype)
@@ -202,17 +206,18 @@ def qk_norm_rope(query, key, query_weight, key_weight, cos, sin, positions=None,
             raise ValueError(f"{what}: {name} must be on {device}, got {t.device}")
         if t.requires_grad:
             raise NotImplementedError(f"{what}: the angle tables take no gradient")
-        tables.append(t.to(table).contiguous())
+        tables.append(t if t.dtype == table and t.is_contiguous() else t.to(table).contiguous())
     if positions is None:
         if T > cos.shape[0]:
             raise IndexError(f"{what}: {T} tokens need {T} table rows, got {cos.shape[0]}")
     else:
         _check_index_tensor(f"{what}: positions", positions, device, cls)
-        if tuple(positions.shape) not in ((T,), (B, T)):
+        if positions.shape != (T,) and positions.shape != (B, T):
             raise ValueError(f"{what}: positions must be ({T},) or ({B}, {T}), got {tuple(positions.shape)}")
         if check_indices:
             K._check_indices(positions, cos.shape[0], f"{what} position")
-        positions = positions.to(torch.int64).contiguous()
+        if positions.dtype != torch.int64 or not positions.is_contiguous():
+            positions = positions.to(torch.int64).contiguous()
     plan = (*tables, positions, float(eps), bool(interleaved))
     planes = [_full(planes[0], degree), _full(planes[1], degree), planes[2], planes[3]]
     if _wants_grad(query, key, query_weight, key_weight):
@@ -364,7 +369,8 @@ def token_log_probs(logits, tokens, top=0, temperature=1.0, ignore_index=-100, c
     ignore_index = operator.index(ignore_index)
     if check_indices:
         K._check_indices(tokens, V, f"{what} token", ignore=ignore_index)
-    tokens = tokens.to(torch.int64)
+    if tokens.dtype != torch.int64:
+        tokens = tokens.to(torch.int64)
     if len(lead) != 1:
         planes, tokens = [z.reshape(-1, V) for z in planes], tokens.reshape(-1)
     scale = 1.0 / temperature
