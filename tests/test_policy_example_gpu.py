@@ -31,12 +31,16 @@ def test_first_plane_is_the_derivative_by_the_bonus(example):
         return model, loss
 
     (near, loss), (far, _) = after(0.01), after(1.01)
+    start = example.Decoder(vocab=96, width=128, heads=2, layers=2, degree=1, positions=40)
     assert len(loss) == 2 and loss[1] < 0     # d loss / d bonus = -entropy
     for name, w in near.p.items():
         moved = far.p[name].coeffs[0].double() - near.p[name].coeffs[0].double()
         got = w.coeffs[1].double()
-        # float32 weights of size w: their difference carries 2^-23 |w| of rounding, the products 2^-15
-        room = 2.0 ** -22 * w.coeffs[0].double().norm() + 2.0 ** -12 * got.norm()
+        # float32 weights of size w: their difference carries 2^-23 |w| of rounding; a gradient through a
+        # few float32 products (2^-16 each) carries 2^-14 of its size, in both runs, of which the part that
+        # the bonus does not enter is the step taken with almost none
+        step = (w.coeffs[0].double() - start.p[name].coeffs[0].double()).norm()
+        room = 2.0 ** -22 * w.coeffs[0].double().norm() + 2.0 ** -12 * got.norm() + 2.0 ** -13 * step
         assert (got - moved).norm() <= room, name
 
 
