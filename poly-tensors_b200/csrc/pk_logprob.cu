@@ -54,6 +54,18 @@ __device__ __forceinline__ float exp_fast(float x) {
     return y;
 }
 __device__ __forceinline__ double exp_fast(double x) { return exp(x); }
+// exp of two values.  (The difference z - m comes first and is scaled to base 2 after: folding log2 e into the
+// difference would round m log2 e, which shows when logits are large.)
+__device__ __forceinline__ void exp_both(Two<float> d, float& w0, float& w1) {
+    float a, b;
+    (d * Two<float>(1.4426950408889634f)).get(a, b);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w0) : "f"(a));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w1) : "f"(b));
+}
+__device__ __forceinline__ void exp_both(Two<double> d, double& w0, double& w1) {
+    w0 = exp(d.lo);
+    w1 = exp(d.hi);
+}
 // the same with subnormal results (a gradient of 1e-38 is one; a weight of 1e-38 beside a sum of 1 is not)
 __device__ __forceinline__ float exp_small(float x) {
     float y;
@@ -69,6 +81,31 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 __device__ __forceinline__ double max_nan(double a, double b) { return a != a ? a : b != b ? b : fmax(a, b); }
+
+// The largest of a vector's elements (16-bit ones are compared in pairs as they are stored).
+template <typename T, int VEC, typename C>
+__device__ __forceinline__ C largest_of(const Raw<T, VEC>& v) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        __nv_bfloat162 t = *reinterpret_cast<const __nv_bfloat162*>(&v.w[0]);
+#pragma unroll
+        for (int i = 1; i < VEC / 2; ++i) t = __hmax2_nan(t, *reinterpret_cast<const __nv_bfloat162*>(&v.w[i]));
+        return max_nan(__low2float(t), __high2float(t));
+    } else if constexpr (std::is_same<T, __half>::value) {
+        __half2 t = *reinterpret_cast<const __half2*>(&v.w[0]);
+#pragma unroll
+        for (int i = 1; i < VEC / 2; ++i) t = __hmax2_nan(t, *reinterpret_cast<const __half2*>(&v.w[i]));
+        return max_nan(__low2float(t), __high2float(t));
+    } else {
+        C top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) {
+            C a, b;
+            v.get(i).get(a, b);
+            top = max_nan(top, max_nan(a, b));
+        }
+        return top;
+    }
+}
 
 // Elements of a 16-byte vector.
 template <typename T>
@@ -97,15 +134,15 @@ struct Group {
     Raw<T, VEC> v[NP];
 
     __device__ __forceinline__ void load(const LogProbParams& p, int64_t row_at, const RowGroups& row, int g) {
-        const int64_t first = static_cast<int64_t>(g) * VEC - row.skew;
         if (row.whole(g)) {
 #pragma unroll
             for (int k = 0; k < NP; ++k) {
                 if constexpr (NP > 6) v[k] = Raw<T, VEC>{};
                 if (NP <= 6 || k < p.np)
-                    v[k] = *reinterpret_cast<const Raw<T, VEC>*>(static_cast<const T*>(p.x[k]) + row_at + first);
+                    v[k] = reinterpret_cast<const Raw<T, VEC>*>(static_cast<const T*>(p.x[k]) + (row_at - row.skew))[g];
             }
         } else {
+            const int64_t first = static_cast<int64_t>(g) * VEC - row.skew;
 #pragma unroll
             for (int k = 0; k < NP; ++k) {
 #pragma unroll
@@ -164,13 +201,16 @@ struct LogSum {
         }
         m = to;
     }
-    // Two elements: z holds the constant planes unscaled, u the directions scaled (u[0] unused).
+    // Two elements: x holds the constant planes unscaled, u the directions scaled (u[0] unused).
     __device__ __forceinline__ void add(Two<C> x, C scale, Two<C> (&u)[NP]) {
         Two<C> d = fma2(x, Two<C>(scale), Two<C>(m == -INFINITY ? C(0) : -m));
-        C d0, d1;
+        C d0, d1, w0, w1;
         d.get(d0, d1);
-        const C w0 = exp_fast(d0), w1 = exp_fast(d1);
-        if (w0 == C(0) || w1 == C(0)) {
+        exp_both(d, w0, w1);
+        if constexpr (NP == 1) {
+            // masked logits: any finite difference does, its weight is 0
+            d = Two<C>(fmax(d0, C(-1000)), fmax(d1, C(-1000)));
+        } else if (w0 == C(0) || w1 == C(0)) {
             // masked, or too far below the maximum to count: neither its logit nor its directions enter
             d = Two<C>(w0 == C(0) ? C(0) : d0, w1 == C(0) ? C(0) : d1);
 #pragma unroll
@@ -391,11 +431,20 @@ constexpr int lp_depth() { return NP == 1 || (NP == 2 && sizeof(T) == 4 && !TOP)
 template <int NP>
 constexpr int lp_threads() { return NP > 3 ? 256 : 512; }
 
+// Blocks per SM that the registers have to leave room for, where the compiler would take more than pays: 64 or
+// 80 registers a thread (8192 x 32000 bfloat16, degree 1: 247 us with the 72 that it takes unasked, 233 with 64).
+template <typename T, int NP, bool TOP>
+constexpr int lp_blocks() {
+    if (sizeof(T) == 8) return 1;
+    if (NP == 4) return 3;
+    return (NP <= 3 && TOP) || (NP == 2 && sizeof(T) == 2) ? 2 : 1;
+}
+
 // One pass over the logits: the blocks of a cluster (gridDim.x of them, one or more) share a row, each
 // thread keeps the running sums of its groups of 16 bytes per plane, and the parts are joined in the warp,
 // in the block and through distributed shared memory in the cluster's first block.
 template <typename T, int NP, bool TOP>
-__global__ void __launch_bounds__(lp_threads<NP>(), sizeof(T) == 8 ? 1 : NP == 4 ? 3 : NP <= 3 && TOP ? 2 : 1)
+__global__ void __launch_bounds__(lp_threads<NP>(), lp_blocks<T, NP, TOP>())
 token_log_probs_fwd_kernel(const __grid_constant__ LogProbParams p) {
     using C = typename Compute<T>::type;
     constexpr int VEC = lp_vec<T>(), DEPTH = lp_depth<T, NP, TOP>();
@@ -452,12 +501,7 @@ token_log_probs_fwd_kernel(const __grid_constant__ LogProbParams p) {
             const bool live = g < end;
             C top = -INFINITY;
             if (live) {
-#pragma unroll
-                for (int i = 0; i < VEC / 2; ++i) {
-                    C a, b;
-                    now[d].v[0].get(i).get(a, b);
-                    top = max_nan(top, max_nan(a, b));
-                }
+                top = largest_of<T, VEC, C>(now[d].v[0]);
                 if (top * scale > sum.m + C(LP_SLACK)) sum.raise(top * scale);
 #pragma unroll
                 for (int i = 0; i < VEC / 2; ++i) {
