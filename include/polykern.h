@@ -489,8 +489,9 @@ PK_API int pk_dropout(int dtype, int degree, int64_t n, const void* const* x, in
  *   A logit of -inf is masked: no part in any sum, log probability -inf, no direction.  A row with no
  *   open logit: entropy 0.  A row whose token is ignore_index is not read: zeros, top_tokens -1.  A
  *   token outside [0, cols) gives NaN.
- * pk_token_log_probs_bwd: dlogits from the gradients of log_probs, entropy and top_log_probs (null
- *   arrays: zero), with the forward's stats, entropy and top_tokens.
+ * pk_token_log_probs_bwd: dlogits (row stride dlogits_rs; not the logits' own memory) from the gradients
+ *   of log_probs, entropy and top_log_probs (null arrays: zero), with the forward's stats, entropy and
+ *   top_tokens.
  */
 PK_API int pk_token_log_probs_fwd(int dtype, int degree, int64_t rows, int64_t cols,
                                   const void* const* logits, int64_t logits_rs, const int64_t* tokens,

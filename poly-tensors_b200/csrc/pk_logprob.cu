@@ -12,6 +12,12 @@
 //
 // Sums, maxima and the row series are held in float (double for float64 logits); the results have that
 // type, and the gradient is rounded once to the logits' type when it is stored.
+//
+// Each direction reads the logits once (the forward writes a few numbers per row, the backward the
+// gradient), so memory traffic is the floor.  Measured on B200, device time: 2048 x 32000 float32 degree 3
+// forward 177 us = 5.9 TB/s, backward 336 us = 6.2 TB/s; 8192 rows 645 us = 6.5 TB/s.  16-bit logits are
+// bound by their instructions, about 15 an element at degree 0: 8192 x 32000 bfloat16 126 us = 4.2 TB/s
+// forward; degree 1 233 us = 4.5 TB/s; five alternatives add 54 us to the former.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -691,6 +697,8 @@ __device__ __forceinline__ void grad_of(const RowGrad<NP, C>& r, bool has_b, con
     for (int k = 0; k < NP; ++k) out[k] = p0 == C(0) ? C(0) : p0 * out[k];
 }
 
+// The blocks of a row share its groups, about four a thread: enough loads in flight, and few enough blocks that
+// reading the row's own numbers (a dozen) costs little.  There is nothing to join.
 template <typename T, int NP>
 __global__ void __launch_bounds__(256) token_log_probs_bwd_kernel(const __grid_constant__ LogProbParams p) {
     using C = typename Compute<T>::type;
@@ -729,7 +737,8 @@ __global__ void __launch_bounds__(256) token_log_probs_bwd_kernel(const __grid_c
             A[k] = a[k];
         }
         for (int j = 0; j < (p.has_c ? p.top : 0); ++j) {
-            if (to_c<C>(row0[p.top_at[row * p.top + j]]) * scale == -INFINITY) continue;
+            const int64_t at = p.top_at[row * p.top + j];
+            if (at < 0 || at >= p.cols || to_c<C>(row0[at]) * scale == -INFINITY) continue;
 #pragma unroll
             for (int k = 0; k < NP; ++k)
                 if (k < p.np) A[k] += static_cast<const C*>(p.gc[k])[row * p.top + j];

@@ -259,6 +259,19 @@ def test_qk_gradient_by_differences():
             assert abs((up - down) / (2 * h) - want) <= 1e-6 * max(1.0, abs(want)), (which, j)
 
 
+def test_qk_broadcast_heads():
+    """One key head expanded over the groups (stride 0): its gradient is the sum over them."""
+    q, k = heads(2, 5, 4, 1, 64, 0, F64)
+    cos, sin = (t.cuda() for t in tables(5, 32, F64))
+    shared = k[0].clone().requires_grad_()
+    y = api().qk_norm_rope(q[0], shared.expand(2, 5, 4, 64), None, None, cos, sin)[1]
+    g = series((2, 4, 5, 64), 0, 8, F64)[0].cuda()
+    (d,) = torch.autograd.grad(y, shared, g)
+    dense = k[0].expand(2, 5, 4, 64).contiguous().requires_grad_()
+    (e,) = torch.autograd.grad(api().qk_norm_rope(q[0], dense, None, None, cos, sin)[1], dense, g)
+    torch.testing.assert_close(d, e.sum(2, keepdim=True), rtol=1e-13, atol=1e-13)
+
+
 def test_qk_far_rows():
     """Rows more than 2^31 elements apart."""
     gap = (1 << 31) + 64
@@ -641,6 +654,29 @@ def test_log_probs_tokens_out_of_range():
     assert torch.isfinite(got.entropy.coeffs[1]).all()
     (d,) = torch.autograd.grad(got.log_probs, leaf, variable([torch.ones(3, device="cuda"), torch.zeros(3, device="cuda")]))
     assert torch.isnan(d.coeffs[0]).all(1).tolist() == [False, True, True]
+
+
+def test_log_probs_broadcast_rows():
+    """One row of logits for several tokens (row stride 0), and tokens of a narrower integer type."""
+    z = logits(1, 333, 0, F64)[0]
+    one = z.clone().requires_grad_()
+    tokens = random_tokens(4, 333).cuda()
+    got = api().token_log_probs(one.expand(4, 333), tokens.to(torch.int32), top=2)
+    want = api().token_log_probs(z.expand(4, 333).contiguous(), tokens, top=2)
+    assert torch.equal(got.log_probs, want.log_probs) and torch.equal(got.top_tokens, want.top_tokens)
+    (d,) = torch.autograd.grad(got.log_probs.sum(), one)
+    expected = torch.zeros(333, dtype=F64, device="cuda").index_add_(0, tokens, torch.ones(4, dtype=F64, device="cuda"))
+    torch.testing.assert_close(d[0], expected - 4 * torch.softmax(z[0], -1), rtol=1e-12, atol=1e-14)
+
+
+def test_log_probs_changed_logits_are_noticed():
+    """Logits changed in place between forward and backward are an error, not a wrong gradient."""
+    z = logits(2, 50, 1, F32)
+    leaf = variable(z, True)
+    got = api().token_log_probs(leaf, random_tokens(2, 50).cuda())
+    z[1].add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(got.entropy, leaf, variable([torch.ones(2, device="cuda")] + [torch.zeros(2, device="cuda")]))
 
 
 def test_log_probs_no_rows():
