@@ -41,6 +41,7 @@ struct RopeParams {
     const int64_t* positions;           // [b * pos_bs + t], or null: position t
     int64_t pos_bs;
     double eps;
+    int stage_at;                       // backward: where the stages begin in shared memory
 };
 
 // The two features of slot i: rotated pairs first, then the passing features two by two (the second
@@ -595,20 +596,93 @@ __global__ void __launch_bounds__(ROPE_THREADS) qk_norm_rope_fwd_vec_kernel(cons
     }
 }
 
+// What a thread has under way for its next row: its slot of every plane of x and of the gradient and its angles,
+// copied to places in shared memory that only it reads, so that its own wait for the copies is all that
+// orders them.
+template <typename T, int NP, int V>
+struct Stage {
+    using C = typename Compute<T>::type;
+    static constexpr int VB = V * sizeof(T), AB = V * sizeof(C);
+    static constexpr int BYTES = ROPE_THREADS * (4 * NP * VB + 2 * AB);
+    unsigned char* at;
+
+    __device__ __forceinline__ explicit Stage(unsigned char* base) : at(base) {}
+    __device__ __forceinline__ unsigned char* place(int i) const { return at + (i * ROPE_THREADS + threadIdx.x) * VB; }
+    __device__ __forceinline__ C* angle(int i) const {
+        return reinterpret_cast<C*>(at + ROPE_THREADS * 4 * NP * VB + (i * ROPE_THREADS + threadIdx.x) * AB);
+    }
+    template <int BYTES_>
+    static __device__ __forceinline__ void copy(void* to, const void* from) {
+        if constexpr (BYTES_ == 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+        else
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+    }
+    __device__ __forceinline__ void fetch(int first, const void* const* planes, int np, int64_t off, const SlotAt<V>& slot) const {
+#pragma unroll
+        for (int k = 0; k < NP; ++k)
+            if (plane_live<NP>(k, np)) {
+                const T* src = static_cast<const T*>(planes[k]) + off;
+                copy<VB>(place(first + 2 * k), src + slot.a);
+                copy<VB>(place(first + 2 * k + 1), src + slot.b);
+            }
+    }
+    __device__ __forceinline__ void fetch_angles(const RopeParams& p, int64_t pos, int pair) const {
+        const bool inside = pos >= 0 && pos < p.table_rows;
+        if (inside && pair >= 0) {
+            const int64_t from = pos * (p.rotary / 2) + pair;
+#pragma unroll
+            for (int v = 0; v < AB; v += 16) {
+                constexpr int PIECE = AB < 16 ? AB : 16;
+                copy<PIECE>(reinterpret_cast<unsigned char*>(angle(0)) + v, reinterpret_cast<const unsigned char*>(static_cast<const C*>(p.cos_t) + from) + v);
+                copy<PIECE>(reinterpret_cast<unsigned char*>(angle(1)) + v, reinterpret_cast<const unsigned char*>(static_cast<const C*>(p.sin_t) + from) + v);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                angle(0)[j] = inside ? C(1) : C(NAN);
+                angle(1)[j] = inside ? C(0) : C(NAN);
+            }
+        }
+    }
+    __device__ __forceinline__ void read(int first, int np, Slot<NP, T, V>& s, bool inter) const {
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+            if constexpr (NP > 6) s.lo[k] = s.hi[k] = Raw<T, V>{};
+            if (plane_live<NP>(k, np)) {
+                s.lo[k] = *reinterpret_cast<const Raw<T, V>*>(place(first + 2 * k));
+                s.hi[k] = *reinterpret_cast<const Raw<T, V>*>(place(first + 2 * k + 1));
+            }
+        }
+        if (inter) s.part();
+    }
+    __device__ __forceinline__ void read_angles(Angles<V, C>& a) const {
+        C u[V], v[V];
+        load_vec<C, V, C>(angle(0), u);
+        load_vec<C, V, C>(angle(1), v);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            a.c[i] = Two<C>(u[2 * i], u[2 * i + 1]);
+            a.s[i] = Two<C>(v[2 * i], v[2 * i + 1]);
+        }
+    }
+};
+
 // A thread keeps its slot from row to row, so the weight gradient is summed in registers; groups of a
 // warp are joined by shuffles, warps in turn through shared memory, blocks by the weight-sum kernel,
-// always in the same order.
+// always in the same order.  The next row is on its way into shared memory while one is worked on: with the
+// sums in registers too few warps fit an SM to cover the loads by themselves (bfloat16 degree 3 below: 256 us
+// with loads straight into registers, 241 us so), and a row is read from there a second time after its sums.
 //
 // Measured on B200 (4 x 2048 tokens, 2 x 16 heads of 128; bytes are the planes read and written once):
-// forward float32 degree 3 175 us = 6.1 TB/s, bfloat16 degree 3 110 us = 4.9 TB/s; backward 314 us =
-// 5.1 TB/s and 258 us = 3.1 TB/s.  float32 runs near the rate of a copy; the 16-bit backward is
-// bound by its instructions (about 70 packed multiply-adds per pair and the conversions).  Degree 3 needs
-// three blocks per SM to cover its loads (353 us with the two that its 182 registers would allow);
-// asking for more blocks at other degrees spills and loses.
+// forward float32 degree 3 172 us = 6.2 TB/s, bfloat16 degree 3 107 us = 5.0 TB/s; backward 287 us =
+// 5.6 TB/s and 241 us = 3.3 TB/s.  float32 runs near the rate of a copy; the 16-bit backward is
+// bound by its instructions (about 70 packed multiply-adds per pair and the conversions).  Degree 3 asks
+// for three blocks per SM (299 us with the two that its registers would allow); more, or the same at
+// other degrees, spills and loses.
 template <typename T, int NP, int V>
 __global__ void __launch_bounds__(ROPE_THREADS, NP == 4 ? 3 : 1) qk_norm_rope_bwd_vec_kernel(const __grid_constant__ RopeParams p, const RowShape shape, int q_blocks) {
     using C = typename Compute<T>::type;
-    constexpr bool EXACT = std::is_same<T, C>::value;     // storage holds the turned gradient unrounded
     extern __shared__ __align__(16) unsigned char smem[];
     const int lanes = shape.lanes, slots = shape.slots;
     const BlockRows mine(p, q_blocks, lanes);
@@ -627,31 +701,43 @@ __global__ void __launch_bounds__(ROPE_THREADS, NP == 4 ? 3 : 1) qk_norm_rope_bw
 #pragma unroll
         for (int i = 0; i < V / 2; ++i) acc[k][i][0] = acc[k][i][1] = Two<C>(C(0));
     }
-    for (uint32_t first = mine.first; first < mine.rows; first += mine.stride) {
+    using S = Stage<T, NP, V>;
+    unsigned char* stages = smem + p.stage_at;
+    const bool mine_slot = sub < slots;
+    const auto fetch = [&](uint32_t row, int stage) {
+        if (mine_slot && row < mine.rows) {
+            const uint32_t token = shape.by_heads[mine.which].divide(row), h = row - token * mine.heads;
+            const uint32_t b = shape.by_len.divide(token), t = token - b * len;
+            const S s(stages + stage * S::BYTES);
+            s.fetch(0, set.x, p.np, b * set.bs + t * set.ts + h * set.hs, at);
+            s.fetch(2 * NP, set.g, p.np, b * set.g_bs + h * set.g_hs + t * set.g_ts, at);
+            s.fetch_angles(p, position_of(p, b, t), at.angle);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int stage = 0;
+    fetch(mine.first + threadIdx.x / lanes, 0);
+    for (uint32_t first = mine.first; first < mine.rows; first += mine.stride, stage ^= 1) {
         const uint32_t row = first + threadIdx.x / lanes;
-        const bool live = sub < slots && row < mine.rows;
-        const uint32_t token = shape.by_heads[mine.which].divide(row), h = row - token * mine.heads;
-        const uint32_t b = shape.by_len.divide(token), t = token - b * len;
+        const bool live = mine_slot && row < mine.rows;
+        fetch(row + mine.stride, stage ^ 1);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        const S here(stages + stage * S::BYTES);
         Slot<NP, T, V> x, g;
         Angles<V, C> angles;
         Two<C> cross[NP], diag[NP], mean[NP];
 #pragma unroll
         for (int k = 0; k < NP; ++k) cross[k] = diag[k] = mean[k] = Two<C>(C(0));
         if (live) {
-            x.load(set.x, p.np, b * set.bs + t * set.ts + h * set.hs, at);
-            g.load(set.g, p.np, b * set.g_bs + h * set.g_hs + t * set.g_ts, at);
-            angles.load(p, position_of(p, b, t), at.angle);
-            if (inter) {
-                x.part();
-                g.part();
-            }
+            here.read(0, p.np, x, inter);
+            here.read(2 * NP, p.np, g, inter);
+            here.read_angles(angles);
 #pragma unroll
             for (int i = 0; i < V / 2; ++i) {
                 Two<C> e[NP], f[NP], u[NP];
                 g.firsts(i, e);
                 g.seconds(i, f);
                 angles.turn(i, true, e, f);
-                if constexpr (EXACT) g.set(i, e, f);
                 weigh<NP, V, C>(weights, set.nw, slots, sub, i, e, f);
                 x.firsts(i, u);
                 pair_square_acc<NP, C>(u, cross, diag);
@@ -681,6 +767,11 @@ __global__ void __launch_bounds__(ROPE_THREADS, NP == 4 ? 3 : 1) qk_norm_rope_bw
             rr[k] = Two<C>(r[k]);
             qq[k] = Two<C>(q[k] * minus);       // -(r (*) r (*) r (*) mean)
         }
+        // read again: what the sums above left no registers for
+        asm volatile("" ::: "memory");
+        here.read(0, p.np, x, inter);
+        here.read(2 * NP, p.np, g, inter);
+        here.read_angles(angles);
 #pragma unroll
         for (int i = 0; i < V / 2; ++i) {
             Two<C> e[2][NP], f[2][NP];
@@ -688,7 +779,7 @@ __global__ void __launch_bounds__(ROPE_THREADS, NP == 4 ? 3 : 1) qk_norm_rope_bw
             x.seconds(i, e[1]);
             g.firsts(i, f[0]);
             g.seconds(i, f[1]);
-            if constexpr (!EXACT) angles.turn(i, true, f[0], f[1]);
+            angles.turn(i, true, f[0], f[1]);
 #pragma unroll
             for (int m2 = 0; m2 < 2; ++m2) {
                 pair_mul<NP, C>(f[m2], rr, f[m2]);          // g' (*) r
@@ -864,8 +955,13 @@ static bool launch_rope_vec(RopeParams& p, const RowShape& row, BwdLaunch* bwd, 
     if (bwd) {
         if constexpr (vec_built(NP, V, sizeof(C), true)) {
             const auto kernel = qk_norm_rope_bwd_vec_kernel<T, NP, V>;
-            bwd->plan<C>(p, resident_blocks(kernel, ROPE_THREADS, weights), rows_per_block);
-            PK_LAUNCHED(kernel<<<bwd->blocks.q + bwd->blocks.k, ROPE_THREADS, weights, s>>>(p, row, bwd->blocks.q));
+            // the weights' place also takes the sums at the end
+            p.stage_at = static_cast<int>(round_up(std::max<int64_t>(weights, static_cast<int64_t>(std::max(bwd->sums[0], bwd->sums[1])) * p.dim * sizeof(C)), 16));
+            const size_t smem = p.stage_at + 2 * static_cast<size_t>(Stage<T, NP, V>::BYTES);
+            if (smem > 48 * 1024)
+                cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+            bwd->plan<C>(p, resident_blocks(kernel, ROPE_THREADS, smem), rows_per_block);
+            PK_LAUNCHED(kernel<<<bwd->blocks.q + bwd->blocks.k, ROPE_THREADS, smem, s>>>(p, row, bwd->blocks.q));
         }
     } else {
         if constexpr (vec_built(NP, V, sizeof(C), false)) {
