@@ -7,7 +7,6 @@ eager-PyTorch fallback.
 """
 
 import ctypes
-import math
 
 import torch
 
@@ -648,14 +647,8 @@ def _dense(planes):
     return planes
 
 
-_SMALL = 1 << 20
-
-
 def _outputs(like, count, shape):
-    """``count`` uninitialised tensors like another: small ones (up to 1 MiB) in one allocation, whose host
-    time would otherwise exceed the kernel's, larger ones each in its own, to be freed one by one."""
-    if math.prod(shape) * like.itemsize <= _SMALL:
-        return list(like.new_empty((count, *shape)).unbind(0))
+    """``count`` uninitialised tensors like another, each with memory of its own."""
     return [like.new_empty(shape) for _ in range(count)]
 
 

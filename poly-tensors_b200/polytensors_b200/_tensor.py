@@ -25,10 +25,6 @@ def _shares_memory(a, b):
     return torch._C._overlaps(a, b)
 
 
-def _pairs_apart(planes):
-    return not any(_shares_memory(planes[i], planes[j]) for i in range(1, len(planes)) for j in range(i))
-
-
 def _is_canonical(planes):
     """True when ``planes`` can be used as they are: plain dense tensors on one device with one
     shape, a floating or complex constant coefficient, every higher coefficient of a single
@@ -43,32 +39,19 @@ def _is_canonical(planes):
         return False
     if len(planes) == 1:
         return True
-    shape, device, direction = head.shape, head.device, None
-    # contiguous planes are told apart by their address ranges, others pair by pair
-    starts = [head.data_ptr()] if head.is_contiguous() else None
+    shape, device = head.shape, head.device
+    direction = planes[1].dtype if isinstance(planes[1], torch.Tensor) else None
+    if direction != kind and direction != _DIRECTION_DTYPE.get(kind):
+        return False
+    storages = {head.untyped_storage()._cdata}
     for c in planes[1:]:
-        if type(c) is not torch.Tensor or c.layout != torch.strided or c.shape != shape or c.device != device:
+        if type(c) is not torch.Tensor or c.layout != torch.strided or c.shape != shape or c.device != device \
+                or c.dtype != direction:
             return False
-        if direction is None:
-            direction = c.dtype
-            if direction != kind and direction != _DIRECTION_DTYPE.get(kind):
-                return False
-        elif c.dtype != direction:
-            return False
-        if starts is not None:
-            if c.is_contiguous():
-                starts.append(c.data_ptr())
-            else:
-                starts = None
-    if starts is not None:
-        starts.sort()
-        size, last = max(head.nbytes, planes[1].nbytes), None
-        for at in starts:
-            if not size or (last is not None and at - last < size):
-                return _pairs_apart(planes)
-            last = at
+        storages.add(c.untyped_storage()._cdata)
+    if len(storages) == len(planes):
         return True
-    return _pairs_apart(planes)
+    return not any(_shares_memory(planes[i], planes[j]) for i in range(1, len(planes)) for j in range(i))
 
 
 def _degree_argument(degree):

@@ -98,3 +98,15 @@ def test_c_entry_refusals():
     assert logp(dtype=4) == -2 and logp(degree=16) == -2 and logp(cols=0) == -1 and logp(rows=-1) == -1
     assert logp(top=33, cols=50) == -1 and logp(top=6) == -1 and logp(z=None) == -1 and logp(rows=0) == 0
     assert "null" in _lib.last_error() or _lib.last_error()
+
+
+def test_constructor_separates_planes_of_one_buffer():
+    """Planes that are views of one buffer, overlapping or not, get memory of their own; separate ones stay."""
+    buffer = torch.randn(4, 6)
+    x = PolyTensor((buffer[0], buffer[1], buffer[1]))
+    assert x.coeffs[0].data_ptr() == buffer[0].data_ptr()
+    assert len({c.untyped_storage().data_ptr() for c in x.coeffs}) == 3
+    apart = (torch.randn(6), torch.randn(6))
+    assert all(a is b for a, b in zip(PolyTensor(apart).coeffs, apart))
+    with pytest.raises(TypeError):
+        PolyTensor((torch.randn(3), "x"))

@@ -746,3 +746,64 @@ def test_log_probs_gradient_by_differences():
             up, down = (objective([p + (s * step if k == n - j else 0) for k, p in enumerate(z)]) for s in (1, -1))
             want = d.coeffs[j][0, i].item()
             assert abs((up - down) / (2 * h) - want) <= 1e-6 * max(1.0, abs(want)), (j, i)
+
+
+# ======================================================================================
+# all of them
+
+def test_calls_in_a_graph():
+    """The forward calls of a decoding step captured in a CUDA graph and replayed on new inputs."""
+    q, k = heads(3, 1, 4, 2, 64, 0, BF16)
+    cos, sin = (t.cuda() for t in tables(50, 32, BF16))
+    positions = torch.tensor([[3], [40], [7]]).cuda()
+    z, tokens = logits(3, 5000, 0, BF16)[0], random_tokens(3, 5000).cuda()
+
+    def step():
+        a, b = api().qk_norm_rope(q[0], k[0], None, None, cos, sin, positions=positions, check_indices=False)
+        got = api().token_log_probs(z, tokens, top=3, check_indices=False)
+        return [a, b, api().dropout(a, 0.5, seed=2), got.log_probs, got.entropy, got.top_log_probs, got.top_tokens]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for t in (q[0], z):
+        t.copy_(torch.randn(t.shape, generator=torch.Generator().manual_seed(12)).to(t.dtype))
+    positions.add_(5)
+    tokens.copy_(random_tokens(3, 5000, seed=9))
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(out, step()):
+        assert torch.equal(a, b)
+
+
+def test_launches_per_call():
+    """One launch forward; backward one, and one more for the weights' sums."""
+    from polytensors_b200 import _lib
+
+    q, k = heads(2, 9, 4, 2, 64, 1, F32)
+    w = weights(64, 1, F32, 5, "series")
+    cos, sin = (t.cuda() for t in tables(9, 32, F32))
+    leaves = [variable(q, True), variable(k, True), variable(w, True), variable(w, True)]
+    counts = []
+
+    def counted(fn):
+        _lib.launch_count(reset=True)
+        out = fn()
+        counts.append(_lib.launch_count())
+        return out
+
+    y = counted(lambda: api().qk_norm_rope(*leaves, cos, sin))
+    seeds = tuple(variable([torch.ones_like(p) for p in t.coeffs]) for t in y)
+    counted(lambda: torch.autograd.grad(y, leaves, seeds))
+    z = variable(logits(3, 100, 1, F32), True)
+    got = counted(lambda: api().token_log_probs(z, random_tokens(3, 100).cuda(), top=2, check_indices=False))
+    ones = variable([torch.ones(3, device="cuda"), torch.zeros(3, device="cuda")])
+    counted(lambda: torch.autograd.grad(got.entropy, z, ones))
+    d = counted(lambda: api().dropout(z, 0.5, seed=1))
+    counted(lambda: torch.autograd.grad(d, z, variable([torch.ones_like(p) for p in d.coeffs])))
+    assert counts == [1, 2, 1, 1, 1, 1]
