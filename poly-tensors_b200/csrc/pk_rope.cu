@@ -616,7 +616,7 @@ struct Stage {
         if constexpr (BYTES_ == 16)
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
         else
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+            asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(to)), "l"(from), "n"(BYTES_) : "memory");
     }
     __device__ __forceinline__ void fetch(int first, const void* const* planes, int np, int64_t off, const SlotAt<V>& slot) const {
 #pragma unroll
@@ -874,14 +874,14 @@ constexpr bool vec_built(int np, int v, int compute_bytes, bool backward) {
     return v >= 2 && held <= (backward ? 48 : 80);
 }
 
-// Vectors of 16 bytes, else of 8, where that form is built, no pair or passing feature is cut, every base
+// Vectors of 16 bytes, else of 8 or 4 (two elements at least), where that form is built, no pair or passing feature is cut, every base
 // and stride is a multiple of the vector, and a row fits a warp; otherwise the scalar form.
 template <typename T, int NP>
 static RowShape row_shape(const RopeParams& p, bool backward) {
     RowShape s;
     constexpr int cb = sizeof(typename Compute<T>::type);
     const int64_t rows = p.batch * p.len * (p.set[0].heads + p.set[1].heads);
-    for (int bytes = 16; bytes >= 8; bytes /= 2) {
+    for (int bytes = 16; bytes >= 2 * static_cast<int>(sizeof(T)) && bytes >= 4; bytes /= 2) {
         const int v = bytes / static_cast<int>(sizeof(T));
         if (!vec_built(NP, v, cb, backward) || p.rotary % (2 * v) || (p.dim - p.rotary) % (2 * v) || p.dim / (2 * v) > 32)
             continue;
@@ -977,8 +977,13 @@ template <typename T, int NP>
 static void launch_rope_np(RopeParams& p, BwdLaunch* bwd, cudaStream_t s) {
     using C = typename Compute<T>::type;
     const RowShape row = row_shape<T, NP>(p, bwd != nullptr);
-    if (launch_rope_vec<T, NP, 16 / sizeof(T)>(p, row, bwd, s) || launch_rope_vec<T, NP, 8 / sizeof(T)>(p, row, bwd, s))
-        return;
+    if (launch_rope_vec<T, NP, 16 / sizeof(T)>(p, row, bwd, s)) return;
+    if constexpr (sizeof(T) <= 4) {
+        if (launch_rope_vec<T, NP, 8 / sizeof(T)>(p, row, bwd, s)) return;
+    }
+    if constexpr (sizeof(T) == 2) {
+        if (launch_rope_vec<T, NP, 2>(p, row, bwd, s)) return;
+    }
     if (bwd) {
         // as many warps as have room for their weight sums in shared memory
         const size_t per_warp = static_cast<size_t>(std::max(bwd->sums[0], bwd->sums[1])) * p.dim * sizeof(C);

@@ -138,6 +138,20 @@ def test_qk_high_degree(n):
     check_qk(1, 5, 2, 2, 16, n, F32)
 
 
+@pytest.mark.parametrize("n", [5, 7, 11, 15])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_qk_high_degree_16_bit(n, dtype):
+    check_qk(1, 5, 3, 1, 32, n, dtype)
+
+
+@pytest.mark.parametrize("D,rotary", [(20, 20), (36, 36), (12, 4), (68, 36), (124, 124)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32, F64])
+def test_qk_narrow_vectors(D, rotary, interleaved, dtype):
+    """Head dimensions that only vectors of four or eight bytes fit."""
+    check_qk(2, 7, 3, 2, D, 1, dtype, rotary=rotary, interleaved=interleaved)
+
+
 @pytest.mark.parametrize("D", [1, 2, 7, 10, 33, 48, 80, 96, 128, 192, 256, 320, 520, 1024])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_qk_head_dimensions(D, dtype):
