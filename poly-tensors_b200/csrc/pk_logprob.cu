@@ -53,33 +53,49 @@ struct LogProbParams {
 constexpr int LP_MAX_TOP = 32;       // a warp's lanes
 constexpr int LP_MAX_SHARE = 8;      // blocks of a row's cluster (the portable limit)
 
-__device__ __forceinline__ float exp_fast(float x) {
-    // 2^(x log2 e) in hardware: the argument's rounding, |x| 2^-24, is the same size as the logit's own
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
-    return y;
+// Largest value, NaN when there is one.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
-__device__ __forceinline__ double exp_fast(double x) { return exp(x); }
-// exp of two values.  (The difference z - m comes first and is scaled to base 2 after: folding log2 e into the
-// difference would round m log2 e, which shows when logits are large.)
+__device__ __forceinline__ double max_nan(double a, double b) { return a != a ? a : b != b ? b : fmax(a, b); }
+
+// exp of two values in hardware, 2^(d log2 e).  (The difference z - m comes first and is scaled to base 2 after:
+// folding log2 e into the difference would round m log2 e, which shows when logits are large.)
+// The product's rounding moves a weight by |d| 2^-24.  That is the size of a logit's own rounding, but the
+// directions' sums take powers of it apart (degree 4: 1.6e-6 in log p's last plane).  float32 logits are bound by
+// memory and take the library's exponential; for 16-bit ones with directions EXP_CAREFUL returns the error: the
+// fused multiply-add gives the product's error r exactly (TwoProduct of Ogita, Rump and Oishi, "Accurate sum and
+// dot product", 2005), and 2^(a + r) = 2^a (1 + r log 2) to first order.
+enum { EXP_PLAIN, EXP_CAREFUL, EXP_LIBRARY };
+template <int HOW>
 __device__ __forceinline__ void exp_both(Two<float> d, float& w0, float& w1) {
+    if constexpr (HOW == EXP_LIBRARY) {
+        float x, y;
+        d.get(x, y);
+        w0 = expf(x);
+        w1 = expf(y);
+        return;
+    }
+    constexpr float LOG2E = 1.4426950408889634f, LOG2 = 0.6931471805599453f;
+    const Two<float> minus = d * Two<float>(-LOG2E);
     float a, b;
-    (d * Two<float>(1.4426950408889634f)).get(a, b);
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w0) : "f"(a));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w1) : "f"(b));
+    minus.get(a, b);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w0) : "f"(-a));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w1) : "f"(-b));
+    if constexpr (HOW == EXP_CAREFUL) {
+        const Two<float> w(w0, w1), r = fma2(d, Two<float>(LOG2E), minus);
+        fma2(w, r * Two<float>(LOG2), w).get(w0, w1);
+    }
 }
+template <int HOW>
 __device__ __forceinline__ void exp_both(Two<double> d, double& w0, double& w1) {
     w0 = exp(d.lo);
     w1 = exp(d.hi);
 }
-// the same with subnormal results (a gradient of 1e-38 is one; a weight of 1e-38 beside a sum of 1 is not)
-__device__ __forceinline__ float exp_small(float x) {
-    float y;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
-    return y;
-}
-__device__ __forceinline__ double exp_small(double x) { return exp(x); }
-// of two values: 2^32 times the result stays normal down to the smallest subnormal one
+// The same with subnormal results (a gradient of 1e-38 is one; a weight of 1e-38 beside a sum of 1 is not): 2^32
+// times the result stays normal down to the smallest of them.
 __device__ __forceinline__ void exp_small_both(Two<float> d, float& w0, float& w1) {
     float a, b;
     fma2(d, Two<float>(1.4426950408889634f), Two<float>(32.0f)).get(a, b);
@@ -88,15 +104,7 @@ __device__ __forceinline__ void exp_small_both(Two<float> d, float& w0, float& w
     w0 = a * 0x1p-32f;
     w1 = b * 0x1p-32f;
 }
-__device__ __forceinline__ void exp_small_both(Two<double> d, double& w0, double& w1) { exp_both(d, w0, w1); }
-
-// Largest value, NaN when there is one.
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ double max_nan(double a, double b) { return a != a ? a : b != b ? b : fmax(a, b); }
+__device__ __forceinline__ void exp_small_both(Two<double> d, double& w0, double& w1) { exp_both<EXP_PLAIN>(d, w0, w1); }
 
 // The largest of a vector's elements (16-bit ones are compared in pairs as they are stored).
 template <typename T, int VEC, typename C>
@@ -187,7 +195,7 @@ constexpr int LP_SLACK = 8;
 // Running state of a part of a row below a reference m (its first largest z_0): S = sum w and
 // T = sum w (*) (z - m), w = exp(z - m).  Two sums of each run side by side (even and odd elements) and are
 // joined at the end.
-template <int NP, typename C>
+template <int NP, typename C, int HOW>
 struct LogSum {
     C m;
     Two<C> S[NP], T[NP];
@@ -198,7 +206,7 @@ struct LogSum {
     }
     // The same sums below a larger m.
     __device__ __forceinline__ void raise(C to) {
-        const C d = m - to, f = m == -INFINITY ? C(0) : exp_fast(d);
+        const C d = m - to, f = m == -INFINITY ? C(0) : c_exp(d);
         if (f == C(0)) {
 #pragma unroll
             for (int k = 0; k < NP; ++k) {
@@ -217,18 +225,19 @@ struct LogSum {
         }
         m = to;
     }
-    // Two elements: x holds the constant planes unscaled, u the directions scaled (u[0] unused).
-    __device__ __forceinline__ void add(Two<C> x, C scale, Two<C> (&u)[NP]) {
+    // Two elements into the sums gs, gt of their group (FIRST: which starts with them).  x holds the constant planes
+    // unscaled, u the directions scaled (u[0] unused).  Group sums first, one addition of them to S and T after:
+    // a quarter or half of the roundings against the running sums, which at degree 3 and 4 show in the entropy's
+    // last planes (2.0e-6 without, 1.1e-6 so) for 1.5 to 4 % of the time.
+    template <bool FIRST>
+    __device__ __forceinline__ void add(Two<C> x, C scale, Two<C> (&u)[NP], Two<C> (&gs)[NP], Two<C> (&gt)[NP]) {
         Two<C> d = fma2(x, Two<C>(scale), Two<C>(m == -INFINITY ? C(0) : -m));
-        C d0, d1, w0, w1;
-        d.get(d0, d1);
-        exp_both(d, w0, w1);
-        if constexpr (NP == 1) {
-            // masked logits: any finite difference does, its weight is 0
-            d = Two<C>(fmax(d0, C(-1000)), fmax(d1, C(-1000)));
-        } else if (w0 == C(0) || w1 == C(0)) {
-            // masked, or too far below the maximum to count: neither its logit nor its directions enter
-            d = Two<C>(w0 == C(0) ? C(0) : d0, w1 == C(0) ? C(0) : d1);
+        C w0, w1;
+        d.get(w0, w1);
+        d = Two<C>(max_nan(w0, C(-1000)), max_nan(w1, C(-1000)));     // masked logits: finite, with a weight of 0
+        exp_both<HOW>(d, w0, w1);
+        if (NP > 1 && (w0 == C(0) || w1 == C(0))) {
+            // masked, or too far below the reference to count: its directions do not enter either
 #pragma unroll
             for (int k = 1; k < NP; ++k) {
                 C a, b;
@@ -239,8 +248,8 @@ struct LogSum {
         const Two<C> w(w0, w1);
         // e = exp(directions) and q = e (*) directions from the same products u_i e_(k-i)
         Two<C> e[NP];
-        S[0] = S[0] + w;
-        T[0] = fma2(w, d, T[0]);
+        gs[0] = FIRST ? w : gs[0] + w;
+        gt[0] = FIRST ? w * d : fma2(w, d, gt[0]);
         e[0] = Two<C>(C(1));
 #pragma unroll
         for (int k = 1; k < NP; ++k) {
@@ -252,8 +261,8 @@ struct LogSum {
                 v = v + o;
             }
             e[k] = t;
-            S[k] = fma2(w, t, S[k]);
-            T[k] = fma2(w, fma2(d, t, v), T[k]);
+            gs[k] = FIRST ? w * t : fma2(w, t, gs[k]);
+            gt[k] = FIRST ? w * fma2(d, t, v) : fma2(w, fma2(d, t, v), gt[k]);
         }
     }
 };
@@ -272,7 +281,7 @@ struct RowSum {
         C top = m;
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, off));
-        const C d = m - top, f = m == -INFINITY ? C(0) : exp_fast(d);
+        const C d = m - top, f = m == -INFINITY ? C(0) : c_exp(d);
 #pragma unroll
         for (int k = 0; k < NP; ++k) {
             T[k] = f == C(0) ? C(0) : f * (T[k] + d * S[k]);
@@ -499,7 +508,7 @@ token_log_probs_fwd_kernel(const __grid_constant__ LogProbParams p) {
     C chosen[NP];                            // the token's logit, asked for now, used at the end
     if (first_block && threadIdx.x == 0 && inside) load_logit<NP, T, C>(p, row, token, chosen);
     const C scale = C(p.scale);
-    LogSum<NP, C> sum;
+    LogSum<NP, C, (sizeof(T) == 4 ? EXP_LIBRARY : NP > 1 ? EXP_CAREFUL : EXP_PLAIN)> sum;
     sum.clear();
     C largest = -INFINITY, second = -INFINITY;      // of the thread's groups (NaN above all), and
     int where = begin + threadIdx.x;                // the group of the first
@@ -519,6 +528,7 @@ token_log_probs_fwd_kernel(const __grid_constant__ LogProbParams p) {
             if (live) {
                 top = largest_of<T, VEC, C>(now[d].v[0]);
                 if (top * scale > sum.m + C(LP_SLACK)) sum.raise(top * scale);
+                Two<C> gs[NP], gt[NP];
 #pragma unroll
                 for (int i = 0; i < VEC / 2; ++i) {
                     Two<C> u[NP];
@@ -528,7 +538,13 @@ token_log_probs_fwd_kernel(const __grid_constant__ LogProbParams p) {
 #pragma unroll
                         for (int k = 1; k < NP; ++k) u[k] = u[k] * Two<C>(scale);
                     }
-                    sum.add(now[d].v[0].get(i), scale, u);
+                    if (i == 0) sum.template add<true>(now[d].v[0].get(i), scale, u, gs, gt);
+                    else sum.template add<false>(now[d].v[0].get(i), scale, u, gs, gt);
+                }
+#pragma unroll
+                for (int k = 0; k < NP; ++k) {
+                    sum.S[k] = sum.S[k] + gs[k];
+                    sum.T[k] = sum.T[k] + gt[k];
                 }
             }
             if constexpr (TOP) {
@@ -697,7 +713,7 @@ template <int NP, typename T, typename C>
 __device__ __forceinline__ void grad_of(const RowGrad<NP, C>& r, bool has_b, const C (&z)[NP], C (&out)[NP]) {
     C d[NP], P[NP], q[NP];
     log_prob<NP, C>(z, r.m, r.L, d);
-    const C p0 = z[0] == -INFINITY ? C(0) : exp_small(d[0]);
+    const C p0 = z[0] == -INFINITY ? C(0) : c_exp(d[0]);
     s_exp_dir<NP, C>(d, P);
 #pragma unroll
     for (int k = 0; k < NP; ++k) q[k] = r.G[k];
@@ -784,7 +800,8 @@ __global__ void __launch_bounds__(256) token_log_probs_bwd_kernel(const __grid_c
             C d0, d1;
             d[0].get(d0, d1);
             C p0, p1;
-            exp_small_both(d[0], p0, p1);
+            if constexpr (sizeof(T) == 4) exp_both<EXP_LIBRARY>(d[0], p0, p1);
+            else exp_small_both(d[0], p0, p1);
             if constexpr (NP == 1) d[0] = Two<C>(fmax(d0, C(-1000)), fmax(d1, C(-1000)));   // masked: the weight is 0
             e[0] = Two<C>(C(1));
 #pragma unroll
