@@ -15,9 +15,9 @@
 //
 // Each direction reads the logits once (the forward writes a few numbers per row, the backward the
 // gradient), so memory traffic is the floor.  Measured on B200, device time: 2048 x 32000 float32 degree 3
-// forward 177 us = 5.9 TB/s, backward 336 us = 6.2 TB/s; 8192 rows 645 us = 6.5 TB/s.  16-bit logits are
-// bound by their instructions, about 15 an element at degree 0: 8192 x 32000 bfloat16 126 us = 4.2 TB/s
-// forward; degree 1 233 us = 4.5 TB/s; five alternatives add 54 us to the former.
+// forward 183 us = 5.7 TB/s, backward 338 us = 6.2 TB/s; 8192 rows forward 671 us = 6.3 TB/s.  16-bit logits
+// are bound by their instructions: 8192 x 32000 bfloat16 forward 112 us = 4.7 TB/s at degree 0, 228 us =
+// 4.6 TB/s at degree 1; five alternatives add 48 us to the former.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -898,7 +898,7 @@ static cudaError_t launch_log_probs(const LogProbParams& p, bool backward, cudaS
     while (share < LP_MAX_SHARE && p.rows * share < num_sms() && groups / (2 * share) >= 256) share *= 2;
     int threads = share > 1 && groups / share >= 1024 ? lp_threads<NP>() : groups >= 512 ? 256 : 128;
     // many rows: about sixteen groups a thread, so that a row's join is not most of its work (20000 x 16000
-    // bfloat16 degree 1: 268 us, with four or more 303 us); few rows: more threads, for their latency
+    // bfloat16 degree 1, an earlier build: 268 us, with at least four 303 us); few rows: more threads, for their latency
     if (p.rows >= 8 * num_sms())
         while (threads > 32 && groups < 16 * threads) threads /= 2;
     cudaLaunchConfig_t config{};
