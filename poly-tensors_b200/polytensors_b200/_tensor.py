@@ -43,14 +43,15 @@ def _is_canonical(planes):
     direction = planes[1].dtype if isinstance(planes[1], torch.Tensor) else None
     if direction != kind and direction != _DIRECTION_DTYPE.get(kind):
         return False
-    storages = {head.untyped_storage()._cdata}
     for c in planes[1:]:
         if type(c) is not torch.Tensor or c.layout != torch.strided or c.shape != shape or c.device != device \
                 or c.dtype != direction:
             return False
-        storages.add(c.untyped_storage()._cdata)
-    if len(storages) == len(planes):
-        return True
+    try:
+        if len({c.untyped_storage()._cdata for c in planes}) == len(planes):
+            return True
+    except NotImplementedError:
+        pass                          # a torch.func transform's tensors give out no storage
     return not any(_shares_memory(planes[i], planes[j]) for i in range(1, len(planes)) for j in range(i))
 
 

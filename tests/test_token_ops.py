@@ -110,3 +110,18 @@ def test_constructor_separates_planes_of_one_buffer():
     assert all(a is b for a, b in zip(PolyTensor(apart).coeffs, apart))
     with pytest.raises(TypeError):
         PolyTensor((torch.randn(3), "x"))
+
+
+@pytest.mark.parametrize("same", [False, True])
+def test_constructor_inside_function_transforms(same):
+    """torch.func's tensors have no storage to compare; series of them are built as of any others."""
+    x, y = torch.randn(3, 4), torch.randn(3, 4)
+    build = lambda a, b: PolyTensor((a, a if same else b)).coeffs[1] * 2  # noqa: E731
+    want = 2 * (x if same else y)
+    assert torch.equal(torch.func.vmap(build)(x, y), want)
+    assert torch.equal(torch.func.vmap(torch.func.vmap(build))(x, y), want)
+    dx, dy = torch.func.grad(lambda a, b: build(a, b).sum(), argnums=(0, 1))(x, y)
+    assert torch.equal(dx, torch.full_like(x, 2.0 if same else 0.0))
+    assert torch.equal(dy, torch.full_like(x, 0.0 if same else 2.0))
+    value, tangent = torch.func.jvp(build, (x, y), (torch.ones_like(x), 3 * torch.ones_like(y)))
+    assert torch.equal(value, want) and torch.equal(tangent, torch.full_like(x, 2.0 if same else 6.0))
