@@ -136,9 +136,11 @@ class _QKNormRope(torch.autograd.Function):
     def forward(ctx, query, key, q_weight, k_weight, planes, degree, cls, plan):
         q_out, k_out = K.qk_norm_rope_fwd(*planes, plan)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(*planes[0], *planes[1], *planes[2], *planes[3])
+        # the angles' tensors may be the caller's own: saved, so that a change before backward is noticed
+        angles, ctx.options = [t for t in plan[:3] if t is not None], plan[3:]
+        ctx.save_for_backward(*planes[0], *planes[1], *planes[2], *planes[3], *angles)
         ctx.counts = [len(p) for p in planes]
-        ctx.plan, ctx.degree, ctx.cls = plan, degree, cls
+        ctx.degree, ctx.cls = degree, cls
         ctx.poly = [isinstance(x, cls) for x in (query, key, q_weight, k_weight)]
         return _wrap(q_out, degree, cls), _wrap(k_out, degree, cls)
 
@@ -150,11 +152,13 @@ class _QKNormRope(torch.autograd.Function):
             groups.append(saved[:n])
             del saved[:n]
         Q, Kp, QW, KW = groups
+        cos, sin, *positions = saved
+        plan = (cos, sin, positions[0] if positions else None, *ctx.options)
         GQ, GK = (_grad_planes(g, ctx.degree, ctx.cls) for g in (gq, gk))
         if GQ is None and GK is None:
             return (None,) * 8
         need = ctx.needs_input_grad
-        dq, dk, dqw, dkw = K.qk_norm_rope_bwd(Q, Kp, QW, KW, GQ, GK, ctx.plan, need[2], need[3])
+        dq, dk, dqw, dkw = K.qk_norm_rope_bwd(Q, Kp, QW, KW, GQ, GK, plan, need[2], need[3])
         grads = []
         for planes, poly, wanted in zip((dq, dk, dqw, dkw), ctx.poly, need):
             grads.append(None if planes is None or not wanted else _wrap(planes, ctx.degree if poly else None, ctx.cls))
@@ -221,6 +225,8 @@ def qk_norm_rope(query, key, query_weight, key_weight, cos, sin, positions=None,
     plan = (*tables, positions, float(eps), bool(interleaved))
     planes = [_full(planes[0], degree), _full(planes[1], degree), planes[2], planes[3]]
     if _wants_grad(query, key, query_weight, key_weight):
+        # tensors made in inference mode cannot be saved: a copy can
+        plan = (*[t.clone() if t is not None and t.is_inference() else t for t in plan[:3]], *plan[3:])
         return _QKNormRope.apply(query, key, query_weight, key_weight, planes, degree, cls, plan)
     q_out, k_out = K.qk_norm_rope_fwd(*planes, plan)
     return _wrap(q_out, degree, cls), _wrap(k_out, degree, cls)
