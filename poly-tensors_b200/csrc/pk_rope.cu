@@ -437,9 +437,9 @@ struct Angles {
     }
 };
 
-// Weights of a slot's pair neighbours: first members, second members.
+// Weights of a slot's pair neighbours: first members, second members (16 bytes is what shared memory is declared with).
 template <typename C>
-struct alignas(2 * sizeof(Two<C>)) Weight {
+struct alignas(16) Weight {
     Two<C> lo, hi;
 };
 

@@ -1,4 +1,4 @@
-// Aligned vectors of a storage type in registers, and 16- or 8-byte loads and stores of them.
+// Aligned vectors of a storage type in registers, and loads and stores of them in pieces of 16 bytes at most.
 #pragma once
 
 #include <type_traits>
@@ -7,8 +7,10 @@
 
 namespace pk {
 
+// A vector asks for its own size, for no more than 16 bytes though: longer ones are loaded in pieces, since callers
+// check and lay out memory by 16 bytes (a type's alignment is the compiler's leave to use one wide access).
 template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
+struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Vec {
     T e[V];
 };
 

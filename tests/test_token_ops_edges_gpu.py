@@ -53,3 +53,32 @@ def test_qk_angles_of_inference_mode():
     got = gradient()
     cos, sin, positions = (t.clone() for t in (cos, sin, positions))
     assert torch.equal(got, gradient())
+
+
+@pytest.mark.parametrize("offset", [1, 2, 3, 4, 5, 8, 12])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32, F64])
+def test_qk_tables_anywhere_in_their_allocation(dtype, offset):
+    """Tables that start `offset` elements into an allocation (4, 8 or 16 bytes past a wider boundary) give what
+    tables of their own do, forward and backward."""
+    kind = F64 if dtype == F64 else F32
+    angle = torch.arange(9, dtype=F64)[:, None] * 10000.0 ** (-torch.arange(32, dtype=F64) / 32)
+    own = [t.to(kind).cuda() for t in (angle.cos(), angle.sin())]
+    moved = []
+    for t in own:
+        room = torch.empty(offset + t.numel(), dtype=kind, device="cuda")
+        room[offset:].copy_(t.flatten())
+        moved.append(room[offset:].view(t.shape))
+    q, k = (cuda(series((2, 9, h, 64), 1, h, dtype)) for h in (3, 2))
+    w = cuda(series((64,), 1, 5, dtype))
+    gq, gk = (PolyTensor(tuple(cuda(series((2, h, 9, 64), 1, 7 + h, dtype)))) for h in (3, 2))
+
+    def both(cos, sin):
+        leaves = [PolyTensor(tuple(t), requires_grad=True) for t in (q, k, w)]
+        y = PolyTensor.qk_norm_rope(leaves[0], leaves[1], leaves[2], leaves[2], cos, sin)
+        d = torch.autograd.grad(y, leaves, (gq, gk))
+        return [c.detach().double() for t in (*y, *d) for c in t.coeffs]
+
+    # another vector width sums a row in another order: a few roundings of the compute type and the last one
+    unit = {F32: 2.0 ** -23, F64: 2.0 ** -52, BF16: 2.0 ** -7, F16: 2.0 ** -10}[dtype]
+    for a, b in zip(both(*moved), both(*own)):
+        torch.testing.assert_close(a, b, rtol=64 * unit, atol=64 * unit * b.abs().max().item())
