@@ -187,6 +187,7 @@ def fused_cross_entropy(input, target, ignore_index=-100, reduction="mean", soft
     return total / count
 
 
+@K.on_own_device
 def cross_entropy(logits, target, softcap=None, ignore_index=-100, reduction="mean"):
     """PolyTensor.cross_entropy: optional softcap applied inside the fused pass."""
     if cross_entropy_eligible(logits, target, None, reduction, 0.0):
@@ -272,6 +273,7 @@ def linear_cross_entropy_eligible(h, weight, target):
             and planes[0].dtype in (torch.float32, torch.float64) and target.is_cuda)
 
 
+@K.on_own_device
 def linear_cross_entropy(h, weight, target, ignore_index=-100, reduction="mean", softcap=None, chunk_rows=None):
     """Cross entropy of the logits ``h @ weight.T`` (optionally capped as ``softcap * tanh(z / softcap)``)
     without forming all of them: rows go through the linear and the streaming cross-entropy

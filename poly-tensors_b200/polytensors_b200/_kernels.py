@@ -6,7 +6,9 @@ CUDA stream.  Unsupported inputs raise ``NotImplementedError``; there is no CPU 
 eager-PyTorch fallback.
 """
 
+import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -16,8 +18,39 @@ _DTYPE_CODE = {torch.float32: _lib.PK_F32, torch.float64: _lib.PK_F64,
                torch.bfloat16: _lib.PK_BF16, torch.float16: _lib.PK_F16}
 
 
+def elsewhere(device):
+    """Whether a tensor's device is a GPU that is not the thread's current one, where kernels would launch."""
+    return device.type == "cuda" and device.index not in (None, torch.cuda.current_device())
+
+
+_HERE = contextlib.nullcontext()
+
+
+def own_device(operands):
+    """Context that makes the GPU of the first tensor among the operands current: a kernel goes to the current
+    GPU, and handle 0, a GPU's default stream, means the current GPU's."""
+    for x in operands:
+        if isinstance(x, torch.Tensor):
+            return torch.cuda.device(x.device) if elsewhere(x.device) else _HERE
+    return _HERE
+
+
+def on_own_device(fn):
+    """A call that launches kernels, run with its first tensor's GPU current."""
+
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        with own_device((*args, *kwargs.values())):
+            return fn(*args, **kwargs)
+
+    return call
+
+
 def _stream(device):
-    """The handle of the current stream on a device."""
+    """The handle of the current stream on a device, which has to be the thread's current GPU."""
+    if elsewhere(device):
+        raise ValueError(f"tensors on {device} while the current GPU is {torch.cuda.current_device()}: launch inside "
+                         f"torch.cuda.device({device.index})")
     index = device.index
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 

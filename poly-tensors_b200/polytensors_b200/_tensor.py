@@ -16,6 +16,7 @@ import torch
 
 from . import _fused, _state, _token_ops
 from ._dispatch import dispatch
+from ._kernels import own_device
 
 # Complex dtype that may carry the directions of a real constant coefficient.
 _DIRECTION_DTYPE = {torch.float16: torch.complex32, torch.float32: torch.complex64, torch.float64: torch.complex128}
@@ -336,7 +337,8 @@ class PolyTensor(torch.Tensor):
     def __torch_function__(cls, func, types, args=(), kwargs=None):
         kwargs = {} if kwargs is None else kwargs
         if func in _fused.INTERCEPTED:
-            result = _fused.maybe_fused(func, args, kwargs)
+            with own_device((*args, *kwargs.values())):
+                result = _fused.maybe_fused(func, args, kwargs)
             if result is not NotImplemented:
                 return result
         with torch._C.DisableTorchFunctionSubclass():

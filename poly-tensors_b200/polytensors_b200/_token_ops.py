@@ -29,13 +29,14 @@ class TokenLogProbs(NamedTuple):
 
 
 def _public(fn):
-    """A public call: runs with PolyTensor's interception off, so that reading an operand's attributes costs
-    no Python call (the operators handle the planes themselves)."""
+    """A public call: runs on its tensors' GPU and with PolyTensor's interception off, so that reading an
+    operand's attributes costs no Python call (the operators handle the planes themselves)."""
+    on_gpu = K.on_own_device(fn)
 
     @functools.wraps(fn)
     def call(*args, **kwargs):
         with torch._C.DisableTorchFunctionSubclass():
-            return fn(*args, **kwargs)
+            return on_gpu(*args, **kwargs)
 
     return call
 
