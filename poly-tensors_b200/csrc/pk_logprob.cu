@@ -299,20 +299,24 @@ struct RowSum {
     }
 };
 
+// One logit: the constant plane as stored, the directions scaled.
 template <int NP, typename T, typename C>
-__device__ __forceinline__ void load_logit(const LogProbParams& p, int64_t row, int64_t col, C (&z)[NP]) {
+__device__ __forceinline__ void load_logit(const LogProbParams& p, int64_t row, int64_t col, C (&x)[NP]) {
 #pragma unroll
-    for (int k = 0; k < NP; ++k)
-        z[k] = k < p.np ? to_c<C>(static_cast<const T*>(p.x[k])[row * p.x_rs + col]) * C(p.scale) : C(0);
+    for (int k = 0; k < NP; ++k) {
+        x[k] = k < p.np ? to_c<C>(static_cast<const T*>(p.x[k])[row * p.x_rs + col]) : C(0);
+        if (k) x[k] *= C(p.scale);
+    }
 }
 
-// log probability series of one logit
+// Log probability series of one logit.  z - m is one rounding of scale * x - m, as in the sums and the gradient: a
+// product rounded by itself would stand in full (2e-6 at |z| = 40) in a log probability near 0.
 template <int NP, typename C>
-__device__ __forceinline__ void log_prob(const C (&z)[NP], C m, const C (&L)[NP], C (&out)[NP]) {
-    const bool masked = z[0] == -INFINITY;
-    out[0] = masked ? C(-INFINITY) : (z[0] - m) - L[0];
+__device__ __forceinline__ void log_prob(const C (&x)[NP], C scale, C m, const C (&L)[NP], C (&out)[NP]) {
+    const bool masked = x[0] * scale == -INFINITY;
+    out[0] = masked ? C(-INFINITY) : fma(x[0], scale, -m) - L[0];
 #pragma unroll
-    for (int k = 1; k < NP; ++k) out[k] = masked ? C(0) : z[k] - L[k];
+    for (int k = 1; k < NP; ++k) out[k] = masked ? C(0) : x[k] - L[k];
 }
 
 // A logit and its index as one key: a larger key is a larger logit, or the same with a lower index.  NaN
@@ -677,7 +681,7 @@ token_log_probs_fwd_kernel(const __grid_constant__ LogProbParams p) {
     if (TOP && lane < p.top) {
         C z[NP], v[NP];
         load_logit<NP, T, C>(p, row, best.mine.at(), z);
-        log_prob<NP, C>(z, m, L, v);
+        log_prob<NP, C>(z, scale, m, L, v);
         p.top_tokens[row * p.top + lane] = best.mine.at();
 #pragma unroll
         for (int k = 0; k < NP; ++k)
@@ -685,7 +689,7 @@ token_log_probs_fwd_kernel(const __grid_constant__ LogProbParams p) {
     }
     if (lane == 0) {
         C v[NP], E[NP];
-        if (inside) log_prob<NP, C>(chosen, m, L, v);
+        if (inside) log_prob<NP, C>(chosen, scale, m, L, v);
         s_div<NP, C>(all.T, all.S, E);
         C* stats = static_cast<C*>(p.stats) + row * (p.np + 1);
         stats[0] = m;
@@ -710,10 +714,10 @@ struct RowGrad {
 };
 
 template <int NP, typename T, typename C>
-__device__ __forceinline__ void grad_of(const RowGrad<NP, C>& r, bool has_b, const C (&z)[NP], C (&out)[NP]) {
+__device__ __forceinline__ void grad_of(const RowGrad<NP, C>& r, C scale, bool has_b, const C (&x)[NP], C (&out)[NP]) {
     C d[NP], P[NP], q[NP];
-    log_prob<NP, C>(z, r.m, r.L, d);
-    const C p0 = z[0] == -INFINITY ? C(0) : c_exp(d[0]);
+    log_prob<NP, C>(x, scale, r.m, r.L, d);
+    const C p0 = d[0] == -INFINITY ? C(0) : c_exp(d[0]);
     s_exp_dir<NP, C>(d, P);
 #pragma unroll
     for (int k = 0; k < NP; ++k) q[k] = r.G[k];
@@ -855,8 +859,8 @@ __global__ void __launch_bounds__(256) token_log_probs_bwd_kernel(const __grid_c
     if (at < 0 || at >= p.cols || at < low || at >= high) return;
     C z[NP], o[NP];
     load_logit<NP, T, C>(p, row, at, z);
-    if (z[0] == -INFINITY) return;               // masked: the 0 stands
-    grad_of<NP, T, C>(r, p.has_b != 0, z, o);
+    if (z[0] * scale == -INFINITY) return;       // masked: the 0 stands
+    grad_of<NP, T, C>(r, scale, p.has_b != 0, z, o);
     if (at == token) {
 #pragma unroll
         for (int k = 0; k < NP; ++k) o[k] += scale * a[k];

@@ -9,6 +9,8 @@ from polytensors_b200 import PolyTensor
 pytestmark = pytest.mark.gpu
 
 F32, F64, BF16, F16 = torch.float32, torch.float64, torch.bfloat16, torch.float16
+U = 2.0 ** -24          # unit roundoff of the sums
+OUT = {F32: 2.0 ** -24, BF16: 2.0 ** -8, F16: 2.0 ** -11}
 
 
 @pytest.fixture(autouse=True)
@@ -82,3 +84,60 @@ def test_qk_tables_anywhere_in_their_allocation(dtype, offset):
     unit = {F32: 2.0 ** -23, F64: 2.0 ** -52, BF16: 2.0 ** -7, F16: 2.0 ** -10}[dtype]
     for a, b in zip(both(*moved), both(*own)):
         torch.testing.assert_close(a, b, rtol=64 * unit, atol=64 * unit * b.abs().max().item())
+
+
+# ======================================================================================
+# one word holds nearly all of a row
+
+GAPS = (4.0, 4.7, 5.3, 6.0, 6.6, 7.1, 7.6, 7.9)
+
+
+def peaked(dtype, V, base, far, scale=1.0):
+    """Rows of two open words 512 groups of 16 bytes apart, the later one GAPS above the earlier; the rest at ``far``."""
+    apart = 8192 // dtype.itemsize
+    z = torch.full((len(GAPS), V), far, dtype=F64)
+    z[:, 5] = base
+    z[:, 5 + apart] = base + torch.tensor(GAPS, dtype=F64) * scale
+    return z.to(dtype), 5 + apart
+
+
+def check_peaked(z, top, temperature, n):
+    """With m the row's largest logit and s the other word's weight, S = 1 + s is rounded at most twice (2 u), the
+    weight s carries at most 20 u of its own size (difference, exponential, rescaling), and a temperature
+    leaves up to 2 u more on S (the largest logit's own difference from its rounded value):
+      log p:  5 u + 25 u s,        entropy: the same, 30 u |E| of E = sum p (z - m) and its last rounding,
+      d entropy / dz at the word: p |log p + H| = p |E - (z - m)|, where L cancels: 2 u H + 45 u |E|,
+      d log p / dz: 1 - p, p = exp(log p) with log p's bound, 4 u of the exponential, one rounding."""
+    dtype, rows = z.dtype, z.shape[0]
+    zeros = [torch.zeros_like(z) for _ in range(n)]
+    x = torch.nn.Parameter(z.cuda()) if n == 0 else PolyTensor((z.cuda(), *[t.cuda() for t in zeros]), requires_grad=True)
+    got = PolyTensor.token_log_probs(x, torch.full((rows,), top).cuda(), temperature=temperature)
+    first = lambda t: (t.coeffs[0] if n else t).detach().cpu().double()  # noqa: E731
+    w = z.double() / temperature
+    d = w - w[:, top:top + 1]
+    weight = d.exp()
+    rest = weight.clone()
+    rest[:, top] = 0
+    s = rest.sum(1)
+    logp = -torch.log1p(s)
+    E = torch.where(rest > 0, rest * d, torch.zeros_like(d)).sum(1) / (1 + s)
+    H = -logp - E
+    room = 5 * U + 25 * U * s
+    assert ((first(got.log_probs) - logp).abs() <= room).all()
+    assert ((first(got.entropy) - H).abs() <= room + 30 * U * E.abs() + U * H).all()
+    one = torch.ones(rows, device="cuda")
+    one = PolyTensor((one,), degree=n) if n else one
+    (dh,) = torch.autograd.grad(got.entropy, x, one, retain_graph=True)
+    want = logp.exp() * -(logp + H) / temperature
+    room = (2 * U * H + 45 * U * E.abs()) / temperature + OUT[dtype] * want.abs()
+    assert ((first(dh)[:, top] - want).abs() <= room).all()
+    (da,) = torch.autograd.grad(got.log_probs, x, one)
+    want = -torch.expm1(logp) / temperature
+    assert ((first(da)[:, top] - want).abs() <= 12 * U / temperature + OUT[dtype] * want.abs()).all()
+
+
+@pytest.mark.parametrize("n", [0, 2])
+@pytest.mark.parametrize("base", [40.3, -61.7])
+def test_log_probs_of_confident_rows_at_a_temperature(base, n):
+    """logit / temperature is not a float32 number; its rounding must not stand in a log probability near 0."""
+    check_peaked(*peaked(F32, 5003, base, -float("inf"), scale=0.7), 0.7, n)
