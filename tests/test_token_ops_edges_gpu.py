@@ -136,6 +136,16 @@ def check_peaked(z, top, temperature, n):
     assert ((first(da)[:, top] - want).abs() <= 12 * U / temperature + OUT[dtype] * want.abs()).all()
 
 
+@pytest.mark.parametrize("far", [-float("inf"), -60.0])
+@pytest.mark.parametrize("dtype,V", [(F32, 32000), (F32, 5003), (BF16, 32000), (F16, 9000), (F32, 20011), (BF16, 60000),
+                                     (F16, 61003)])
+@pytest.mark.parametrize("n", [0, 2])
+def test_log_probs_of_confident_rows(dtype, V, far, n):
+    """A later word of the same thread stands 4 to 8 above the first: what is left of its log probability and
+    of the entropy is of the size of the other word's weight, not of the gap."""
+    check_peaked(*peaked(dtype, V, 0.375, far), 1.0, n)
+
+
 @pytest.mark.parametrize("n", [0, 2])
 @pytest.mark.parametrize("base", [40.3, -61.7])
 def test_log_probs_of_confident_rows_at_a_temperature(base, n):
