@@ -172,6 +172,8 @@ using namespace pk;
 extern "C" int pk_dropout(int dtype, int degree, int64_t n, const void* const* x, int x_planes,
                           const void* const* residual, int residual_planes, uint64_t threshold, double scale,
                           uint64_t seed, uint64_t offset, void* const* y, void* stream) {
+    if (dtype != PK_F32 && dtype != PK_F64 && dtype != PK_BF16 && dtype != PK_F16)
+        return fail(PK_ERR_UNSUPPORTED, "pk_dropout: unsupported dtype");
     if (degree < 0 || degree >= PK_MAX_PLANES) return fail(PK_ERR_UNSUPPORTED, "pk_dropout: degree out of range");
     if (n < 0) return fail(PK_ERR_ARG, "pk_dropout: negative extent");
     if (threshold > (1ull << 32)) return fail(PK_ERR_ARG, "pk_dropout: threshold beyond 2^32");
@@ -202,8 +204,7 @@ extern "C" int pk_dropout(int dtype, int degree, int64_t n, const void* const* x
         case PK_F32: launch_dropout<float>(p, s); break;
         case PK_F64: launch_dropout<double>(p, s); break;
         case PK_BF16: launch_dropout<__nv_bfloat16>(p, s); break;
-        case PK_F16: launch_dropout<__half>(p, s); break;
-        default: return fail(PK_ERR_UNSUPPORTED, "pk_dropout: unsupported dtype");
+        default: launch_dropout<__half>(p, s); break;
     }
     prof_end("dropout", s, tok);
     PK_CHECK_LAUNCH("pk_dropout");

@@ -125,3 +125,11 @@ def test_constructor_inside_function_transforms(same):
     assert torch.equal(dy, torch.full_like(x, 0.0 if same else 2.0))
     value, tangent = torch.func.jvp(build, (x, y), (torch.ones_like(x), 3 * torch.ones_like(y)))
     assert torch.equal(value, want) and torch.equal(tangent, torch.full_like(x, 2.0 if same else 6.0))
+
+
+def test_c_dropout_refuses_a_type_before_anything_else():
+    """Before its timing events are taken, as the other entry points do; so also without elements."""
+    lib = _lib.load()
+    p, keep = pointers(2)
+    for n in (0, 4):
+        assert lib.pk_dropout(4, 1, n, p, 2, None, 0, 0, 1.0, 0, 0, p, None) == -2
