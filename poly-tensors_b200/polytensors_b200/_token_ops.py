@@ -90,8 +90,7 @@ def _wrap(planes, degree, cls):
     """A kernel's output planes as the caller's kind of variable."""
     if degree is None:
         return planes[0]
-    of = getattr(cls, "_of", cls)       # another PolyTensor class: through its constructor
-    return of(tuple(planes))
+    return cls._of(tuple(planes))
 
 
 def _grad_planes(g, degree, cls):
