@@ -115,9 +115,8 @@ def dispatch(func, args, kwargs):
             "replacing this value with zero would corrupt derivatives.")
     if not polys:
         return func(*args, **kwargs)
-    device = polys[0].coeffs[0].device
-    if K.elsewhere(device):
-        with torch.cuda.device(device):
+    if K.several_gpus() and K.elsewhere(polys[0].coeffs[0].device):
+        with torch.cuda.device(polys[0].coeffs[0].device):
             return dispatch(func, args, kwargs)
     if _state.coefficient_autograd.get():
         return _coefficient_dispatch(func, args, kwargs, polys)

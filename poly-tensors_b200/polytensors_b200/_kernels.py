@@ -6,7 +6,6 @@ CUDA stream.  Unsupported inputs raise ``NotImplementedError``; there is no CPU 
 eager-PyTorch fallback.
 """
 
-import contextlib
 import ctypes
 import functools
 
@@ -18,21 +17,28 @@ _DTYPE_CODE = {torch.float32: _lib.PK_F32, torch.float64: _lib.PK_F64,
                torch.bfloat16: _lib.PK_BF16, torch.float16: _lib.PK_F16}
 
 
+@functools.cache
+def several_gpus():
+    """Whether the process sees more than one GPU (with one, no tensor can lie on another)."""
+    return torch.cuda.device_count() > 1
+
+
 def elsewhere(device):
     """Whether a tensor's device is a GPU that is not the thread's current one, where kernels would launch."""
-    return device.type == "cuda" and device.index not in (None, torch.cuda.current_device())
-
-
-_HERE = contextlib.nullcontext()
+    if not several_gpus():
+        return False
+    index = device.index
+    return index is not None and device.type == "cuda" and index != torch.cuda.current_device()
 
 
 def own_device(operands):
     """Context that makes the GPU of the first tensor among the operands current: a kernel goes to the current
-    GPU, and handle 0, a GPU's default stream, means the current GPU's."""
-    for x in operands:
-        if isinstance(x, torch.Tensor):
-            return torch.cuda.device(x.device) if elsewhere(x.device) else _HERE
-    return _HERE
+    GPU, and handle 0, a GPU's default stream, means the current GPU's.  None where nothing has to change."""
+    if several_gpus():
+        for x in operands:
+            if isinstance(x, torch.Tensor):
+                return torch.cuda.device(x.device) if elsewhere(x.device) else None
+    return None
 
 
 def on_own_device(fn):
@@ -40,7 +46,10 @@ def on_own_device(fn):
 
     @functools.wraps(fn)
     def call(*args, **kwargs):
-        with own_device((*args, *kwargs.values())):
+        other = own_device(args or kwargs.values())
+        if other is None:
+            return fn(*args, **kwargs)
+        with other:
             return fn(*args, **kwargs)
 
     return call

@@ -337,7 +337,7 @@ class PolyTensor(torch.Tensor):
     def __torch_function__(cls, func, types, args=(), kwargs=None):
         kwargs = {} if kwargs is None else kwargs
         if func in _fused.INTERCEPTED:
-            with own_device((*args, *kwargs.values())):
+            with own_device((*args, *kwargs.values())) or contextlib.nullcontext():
                 result = _fused.maybe_fused(func, args, kwargs)
             if result is not NotImplemented:
                 return result

@@ -24,6 +24,7 @@ def gpus(monkeypatch):
         def __exit__(self, *_):
             now[0] = self.before
 
+    monkeypatch.setattr(_kernels, "several_gpus", lambda: True)
     monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
     monkeypatch.setattr(torch.cuda, "device", Device)
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 100 + index)
