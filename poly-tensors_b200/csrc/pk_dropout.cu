@@ -43,7 +43,8 @@ __device__ __forceinline__ uint4 philox4x32_10(uint64_t i, uint64_t offset, uint
     return make_uint4(c0, c1, c2, c3);
 }
 
-// Planes whose bases lie on no 16-byte boundary, and more than 2^34 elements: one thread per counter (four consecutive elements).
+// Planes whose bases lie on no 16-byte boundary, and more than 2^34 elements: one thread per counter (four consecutive
+// elements); 8192 x 4096 degree 0 one element past such a boundary: float32 85 us, bfloat16 69 (53 and 45 on one).
 template <typename T>
 __global__ void __launch_bounds__(256) dropout_scalar_kernel(const DropoutParams p) {
     using C = typename Compute<T>::type;
@@ -72,10 +73,11 @@ constexpr int dropout_unit() { return sizeof(T) == 2 ? 8 : 4; }
 
 // Vector form: a thread asks for its 16-byte vectors of every plane of x and the residual, forms their counters'
 // words while they are on the way (twenty 32 x 32 -> 64-bit products for four elements, whatever the
-// degree), and writes.  Measured on B200, device time, without a residual: 8192 x 4096 float32 degree 3 158 us
-// = 6.8 TB/s and float64 degree 0 81 us = 6.6 TB/s, the rate of a copy; bfloat16 degree 3 87 us = 6.2 TB/s.  At
-// degree 0 the products are the limit for 16-bit planes: 47 us = 2.8 TB/s (74 % of the issue slots, the multiplier
-// pipe full), where the bytes alone would take 21 us.
+// degree), and writes.  Measured on B200, device time, without a residual: 8192 x 4096 float32 degree 3 159 us
+// = 6.8 TB/s and float64 degree 0 80 us = 6.7 TB/s, the rate of a copy; bfloat16 degree 3 84 us = 6.4 TB/s.  At
+// degree 0 the instructions are the limit for 16-bit planes: 46 us = 2.9 TB/s, where the bytes alone would take
+// 21 us (74 % of the issue slots, the integer pipe 47 %, the multiplier's 38 %; of 237 instructions per eight elements
+// the generator has about 90, the rest is conversion, masking and addresses).
 template <typename T, int NP>
 __global__ void __launch_bounds__(256) dropout_vec_kernel(const __grid_constant__ DropoutParams p) {
     using C = typename Compute<T>::type;

@@ -16,9 +16,13 @@
 //
 // Each direction reads the logits once (the forward writes a few numbers per row, the backward the
 // gradient), so memory traffic is the floor.  Measured on B200, device time: 2048 x 32000 float32 degree 3
-// forward 183 us = 5.7 TB/s, backward 338 us = 6.2 TB/s; 8192 rows forward 671 us = 6.3 TB/s.  16-bit logits
-// are bound by their instructions: 8192 x 32000 bfloat16 forward 112 us = 4.7 TB/s at degree 0, 228 us =
-// 4.6 TB/s at degree 1; five alternatives add 48 us to the former.
+// forward 182 us = 5.8 TB/s, backward 337 us = 6.2 TB/s; 8192 rows forward 666 us = 6.3 TB/s.  16-bit logits at
+// degree 0 and 1 and 64-bit ones are held up by their instructions: 8192 x 32000 bfloat16 forward 114 us = 4.6 TB/s at
+// degree 0 (68 % of the issue slots, the exponentials' pipe 50 %, the integer pipe 48 %), 236 us = 4.5 TB/s at
+// degree 1; five alternatives add 53 us to the former (a search and a merge per row behind two block barriers, with
+// none of the next row's loads under way); 1024 x 32000 float64 degree 2 forward 189 us = 4.2 TB/s (58 % of the issue
+// slots, the double-precision pipe 40 %, 22 % of the warps active: waits between dependent operations), backward 290 us =
+// 5.4 TB/s; 300 x 8191 45 and 30 us, where the bytes alone would take 9 and 18.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -471,12 +475,13 @@ template <int NP>
 constexpr int lp_threads() { return NP > 3 ? 256 : 512; }
 
 // Blocks per SM that the registers have to leave room for, where the compiler would take more than pays: 64 or
-// 80 registers a thread (8192 x 32000 bfloat16, degree 1: 247 us with the 72 that it takes unasked, 233 with 64).
+// 80 registers a thread (1511 x 50021 bfloat16, degree 1, masked words, four alternatives: 120 us unasked, 102 so;
+// 2048 x 32000 float32, degree 3: 198 and 182 us).
 template <typename T, int NP, bool TOP>
 constexpr int lp_blocks() {
     if (sizeof(T) == 8) return 1;
     if (NP == 4) return 3;
-    return (NP <= 3 && TOP) || (NP == 2 && sizeof(T) == 2) ? 2 : 1;
+    return NP <= 3 && TOP ? 2 : 1;
 }
 
 // One pass over the logits: the blocks of a cluster (gridDim.x of them, one or more) share a row, each
@@ -917,7 +922,7 @@ static cudaError_t launch_log_probs(const LogProbParams& p, bool backward, cudaS
     while (share < LP_MAX_SHARE && p.rows * share < num_sms() && groups / (2 * share) >= 256) share *= 2;
     int threads = share > 1 && groups / share >= 1024 ? lp_threads<NP>() : groups >= 512 ? 256 : 128;
     // many rows: about sixteen groups a thread, so that a row's join is not most of its work (20000 x 16000
-    // bfloat16 degree 1, an earlier build: 268 us, with at least four 303 us); few rows: more threads, for their latency
+    // bfloat16 degree 1: 291 us, with at least four 330 us); few rows: more threads, for their latency
     if (p.rows >= 8 * num_sms())
         while (threads > 32 && groups < 16 * threads) threads /= 2;
     cudaLaunchConfig_t config{};

@@ -334,8 +334,8 @@ struct Slot {
     Raw<T, V> lo[NP], hi[NP];
 
     // All loads are issued before anything reads them: a test between two planes' loads makes the second
-    // wait for the first (measured so: 837 instead of 403 us at 4 x 2048 tokens, 2 x 16 heads of 128,
-    // degree 3, float32 backward).
+    // wait for the first (an early build, without copies ahead: 837 instead of 403 us at 4 x 2048 tokens, 2 x 16
+    // heads of 128, degree 3, float32 backward).
     __device__ __forceinline__ void load(const void* const* planes, int np, int64_t off, const SlotAt<V>& at) {
 #pragma unroll
         for (int k = 0; k < NP; ++k) {
@@ -672,14 +672,16 @@ struct Stage {
 // warp are joined by shuffles, warps in turn through shared memory, blocks by the weight-sum kernel,
 // always in the same order.  The next row is on its way into shared memory while one is worked on: with the
 // sums in registers too few warps fit an SM to cover the loads by themselves (bfloat16 degree 3 below: 256 us
-// with loads straight into registers, 241 us so), and a row is read from there a second time after its sums.
+// with loads straight into registers, then 241 us), and a row is read from there a second time after its sums.
 //
 // Measured on B200 (4 x 2048 tokens, 2 x 16 heads of 128; bytes are the planes read and written once):
-// forward float32 degree 3 172 us = 6.2 TB/s, bfloat16 degree 3 107 us = 5.0 TB/s; backward 287 us =
-// 5.6 TB/s and 241 us = 3.3 TB/s.  float32 runs near the rate of a copy; the 16-bit backward is
-// bound by its instructions (about 70 packed multiply-adds per pair and the conversions).  Degree 3 asks
-// for three blocks per SM (299 us with the two that its registers would allow); more, or the same at
-// other degrees, spills and loses.
+// forward float32 degree 3 172 us = 6.2 TB/s, bfloat16 degree 3 106 us = 5.1 TB/s; backward 292 us =
+// 5.5 TB/s and 241 us = 3.3 TB/s.  float32 runs near the rate of a copy.  The 16-bit backward is held up by latency:
+// at 152 registers 17 % of the warps are active, and no pipe is near full (issue slots 54 %, L1 50 %, FMA 45 %).
+// At degree 0 the angles are most of what a row reads, again for each of a token's heads: forward 40 us = 3.4 TB/s
+// (issue 66 %, L1 58 %), backward 75 us = 2.7 TB/s (L1 68 %, waits for shared memory).  Degree 3 asks for three
+// blocks per SM (float32 300 us with the two that its registers would allow; bfloat16 at 4 x 4096 tokens, 32 + 8
+// heads 561, 549 so); more, or the same at other degrees, spills and loses.
 template <typename T, int NP, int V>
 __global__ void __launch_bounds__(ROPE_THREADS, NP == 4 ? 3 : 1) qk_norm_rope_bwd_vec_kernel(const __grid_constant__ RopeParams p, const RowShape shape, int q_blocks) {
     using C = typename Compute<T>::type;
@@ -874,8 +876,10 @@ constexpr bool vec_built(int np, int v, int compute_bytes, bool backward) {
     return v >= 2 && held <= (backward ? 48 : 80);
 }
 
-// Vectors of 16 bytes, else of 8 or 4 (two elements at least), where that form is built, no pair or passing feature is cut, every base
-// and stride is a multiple of the vector, and a row fits a warp; otherwise the scalar form.
+// Vectors of 16 bytes, else of 8 or 4 (two elements at least), where that form is built, no pair or passing feature
+// is cut, every base and stride is a multiple of the vector, and a row fits a warp; otherwise the scalar form, which
+// reads each row twice, element by element (2 x 2048 tokens, 2 x 16 heads of 128, backward: float32 degree 9, where no
+// vector form is built, 2860 us; bfloat16 degree 7 with 4-byte vectors 523 us).
 template <typename T, int NP>
 static RowShape row_shape(const RopeParams& p, bool backward) {
     RowShape s;
