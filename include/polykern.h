@@ -474,7 +474,8 @@ PK_API int pk_qk_norm_rope_bwd(int dtype, int degree, int64_t batch, int64_t len
  * never stored.  Element i (row-major over n contiguous elements) is kept when word i % 4 of
  * Philox4x32-10 with counter (i / 4, offset) and key seed is >= threshold (0 .. 2^32; drop
  * probability threshold / 2^32).  Planes of x and of the residual past x_planes / residual_planes
- * are zero.  A dropped element is 0 whatever x holds.  y may be x or residual.
+ * are zero.  A dropped element is 0 whatever x holds.  y may be x or residual.  seed and offset are part of
+ * the launch: a replayed graph repeats its mask.
  */
 PK_API int pk_dropout(int dtype, int degree, int64_t n, const void* const* x, int x_planes,
                       const void* const* residual, int residual_planes, uint64_t threshold, double scale,

@@ -176,7 +176,8 @@ def qk_norm_rope(query, key, query_weight, key_weight, cos, sin, positions=None,
     where given.  Then feature pair j of the first ``2 * cos.shape[1]`` features turns by the angle of
     its token's position: pairs (j, j + R/2), or adjacent ones with ``interleaved``; the rest pass.
     ``cos`` and ``sin`` (positions, R/2) are ordinary tables; ``positions`` (T,) or (B, T) says which
-    row a token takes (default: 0 .. T-1).
+    row a token takes (default: 0 .. T-1).  Tables and positions that are used as they are (no conversion) and
+    change in place before backward are an error there.
 
     Returns the queries (B, H, T, D) and the keys (B, K, T, D), contiguous: what
     ``scaled_dot_product_attention`` reads.  Positions outside the tables raise IndexError;
@@ -277,7 +278,8 @@ def dropout(input, p, seed, offset=0, residual=None):
 
     The mask is a function of ``seed`` and ``offset`` (ints in [0, 2**64)) and the element's row-major
     index alone (Philox4x32-10 with key ``seed`` and counter (index // 4, offset)); it is not stored,
-    backward forms it again.  Give every dropout of a step its own ``offset`` (or ``seed``).
+    backward forms it again.  Give every dropout of a step its own ``offset`` (or ``seed``).  Both are part of
+    the launch: replays of a captured graph repeat the mask.  ``F.dropout`` is another generator (torch's).
     ``p`` = 0 keeps everything, 1 drops everything.  ``residual`` has the input's shape and type.
     """
     what = "dropout"

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from gpu_util import cuda, series
-from polytensors_b200 import PolyTensor
+from polytensors_b200 import PolyTensor, _state
 
 pytestmark = pytest.mark.gpu
 
@@ -151,3 +151,34 @@ def test_log_probs_of_confident_rows(dtype, V, far, n):
 def test_log_probs_of_confident_rows_at_a_temperature(base, n):
     """logit / temperature is not a float32 number; its rounding must not stand in a log probability near 0."""
     check_peaked(*peaked(F32, 5003, base, -float("inf"), scale=0.7), 0.7, n)
+
+
+# ======================================================================================
+# without plain_range()
+
+def test_default_mode_takes_the_public_coefficients():
+    """Outside plain_range() the operators' results and gradients are those inside it, bit for bit."""
+    angle = torch.arange(9.0)[:, None] * 10000.0 ** (-torch.arange(32.0) / 32)
+    cos, sin, tokens = angle.cos().cuda(), angle.sin().cuda(), torch.arange(18).cuda()
+    inputs = [cuda(series(shape, 2, 20 + i, F32)) for i, shape in enumerate(((2, 9, 4, 64), (2, 9, 2, 64), (64,), (18, 300)))]
+    seeds = [PolyTensor(tuple(cuda(series(shape, 2, 30 + i, F32)))) for i, shape in
+             enumerate(((2, 4, 9, 64), (2, 2, 9, 64), (2, 4, 9, 64), (18,), (18,), (18, 3)))]
+
+    def everything():
+        q, k, w, z = (PolyTensor(tuple(t), requires_grad=True) for t in inputs)
+        a, b = PolyTensor.qk_norm_rope(q, k, w, w, cos, sin)
+        d = PolyTensor.dropout(a, 0.25, seed=3, residual=a)
+        got = PolyTensor.token_log_probs(z, tokens, top=3, temperature=0.9)
+        outs = (a, b, d, *got[:3])
+        grads = torch.autograd.grad(outs, (q, k, w, z), seeds)
+        return [c.detach() for t in (*outs, *grads) for c in t.coeffs]
+
+    inside = everything()                  # the fixture's plain_range()
+    token = _state.plain_range.set(False)
+    _state.exit_plain()
+    try:
+        outside = everything()
+    finally:
+        _state.enter_plain()
+        _state.plain_range.reset(token)
+    assert all(torch.equal(x, y) for x, y in zip(inside, outside))
